@@ -20,6 +20,7 @@
  *     xccl_mc_event_wait and xccl_mem_component_get exist only here.
  */
 #include "xccl_rocm_mem_component.h"
+#include "xccl_rocm_step.h"
 
 #include <dlfcn.h>
 #include <stdio.h>
@@ -28,6 +29,7 @@
 
 static xccl_mem_component_t      *mem_components[UCS_MEMORY_TYPE_LAST];
 static xccl_rocm_mem_component_t *mem_extensions[UCS_MEMORY_TYPE_LAST]; /* NULL: plain reference vtable */
+static const xccl_rocm_step_component_t *mem_steps[UCS_MEMORY_TYPE_LAST]; /* NULL: no optimizer step */
 
 /* UCX v1.10 ucs_memory_type_names[], indexed by ucs_memory_type_t */
 static const char *const memory_type_names[UCS_MEMORY_TYPE_LAST] = {
@@ -68,7 +70,7 @@ xccl_status_t xccl_mem_component_init(const char *components_path)
     const char *cache_env = getenv("XCCL_MEM_COMPONENT_CACHE_SIZE");
     size_t      cache_size = cache_env ? (size_t)strtoull(cache_env, NULL, 0) : 4096;
     size_t      path_len;
-    char       *path, sym[64], *c;
+    char       *path, sym[64], *c; /* the longest name is under 50 bytes */
     void       *handle;
     int         mt;
 
@@ -115,6 +117,14 @@ xccl_status_t xccl_mem_component_init(const char *components_path)
             ext = (xccl_rocm_mem_component_t **)dlsym(handle, sym);
             mem_extensions[mt] = (ext != NULL && *ext != NULL && &(*ext)->super == mc &&
                                   (*ext)->ext_version >= 1) ? *ext : NULL;
+        }
+        {
+            /* likewise the optimizer step, through xccl_<name>_mem_component_step */
+            const xccl_rocm_step_component_t *const *step;
+
+            strcpy(strrchr(sym, '_'), "_step");
+            step          = (const xccl_rocm_step_component_t *const *)dlsym(handle, sym);
+            mem_steps[mt] = (step != NULL && *step != NULL && (*step)->version >= 1) ? *step : NULL;
         }
         mc->dlhandle       = handle;
         mc->cache.size     = cache_size;
@@ -288,6 +298,98 @@ xccl_status_t xccl_mem_component_reduce_multi_nb(void *sbuf1, void *sbuf2, void 
     return st;
 }
 
+/*
+ * The optimizer step (include/xccl_rocm_step.h); no counterpart in the
+ * reference.  An empty event pool is handled as for the reductions above.
+ */
+static xccl_status_t step_of(int mt, const xccl_rocm_step_component_t **step)
+{
+    if (component_of(mt) == NULL) {
+        return XCCL_ERR_UNSUPPORTED;
+    }
+    *step = mem_steps[mt];
+    return *step != NULL ? XCCL_OK : XCCL_ERR_NOT_IMPLEMENTED;
+}
+
+xccl_status_t xccl_mem_component_step_plan_create(const xccl_rocm_step_layout_t *layout,
+                                                  const xccl_rocm_step_tensor_t *tensors, size_t count,
+                                                  ucs_memory_type_t mt, xccl_rocm_step_plan_t **plan)
+{
+    const xccl_rocm_step_component_t *step;
+    xccl_status_t                     st = step_of(mt, &step);
+
+    return st != XCCL_OK ? st : step->plan_create(layout, tensors, count, plan);
+}
+
+xccl_status_t xccl_mem_component_step_plan_destroy(xccl_rocm_step_plan_t *plan, ucs_memory_type_t mt)
+{
+    const xccl_rocm_step_component_t *step;
+    xccl_status_t                     st = step_of(mt, &step);
+
+    return st != XCCL_OK ? st : step->plan_destroy(plan);
+}
+
+xccl_status_t xccl_mem_component_grad_norm(xccl_rocm_step_plan_t *plan, double *stats, ucs_memory_type_t mt)
+{
+    const xccl_rocm_step_component_t *step;
+    xccl_status_t                     st = step_of(mt, &step);
+
+    return st != XCCL_OK ? st : step->grad_norm(plan, stats);
+}
+
+xccl_status_t xccl_mem_component_grad_norm_nb(xccl_rocm_step_plan_t *plan, double *stats, ucs_memory_type_t mt,
+                                              xccl_stream_t *stream, xccl_mc_event_t **event)
+{
+    const xccl_rocm_step_component_t *step;
+    xccl_status_t                     st = step_of(mt, &step);
+
+    if (event != NULL) {
+        *event = NULL;
+    }
+    if (st != XCCL_OK) {
+        return st;
+    }
+    st = step->grad_norm_nb(plan, stats, stream, event);
+    if (st == XCCL_ERR_NO_RESOURCE && stream == NULL) {
+        return step->grad_norm(plan, stats);
+    }
+    if (st == XCCL_OK && event != NULL) {
+        (*event)->mem_type = mt;
+    }
+    return st;
+}
+
+xccl_status_t xccl_mem_component_adamw(xccl_rocm_step_plan_t *plan, const xccl_rocm_adamw_args_t *args,
+                                       ucs_memory_type_t mt)
+{
+    const xccl_rocm_step_component_t *step;
+    xccl_status_t                     st = step_of(mt, &step);
+
+    return st != XCCL_OK ? st : step->adamw(plan, args);
+}
+
+xccl_status_t xccl_mem_component_adamw_nb(xccl_rocm_step_plan_t *plan, const xccl_rocm_adamw_args_t *args,
+                                          ucs_memory_type_t mt, xccl_stream_t *stream, xccl_mc_event_t **event)
+{
+    const xccl_rocm_step_component_t *step;
+    xccl_status_t                     st = step_of(mt, &step);
+
+    if (event != NULL) {
+        *event = NULL;
+    }
+    if (st != XCCL_OK) {
+        return st;
+    }
+    st = step->adamw_nb(plan, args, stream, event);
+    if (st == XCCL_ERR_NO_RESOURCE && stream == NULL) {
+        return step->adamw(plan, args);
+    }
+    if (st == XCCL_OK && event != NULL) {
+        (*event)->mem_type = mt;
+    }
+    return st;
+}
+
 /* reference mem_component.c:150-174: the first component, in memory-type
  * order, that recognises the pointer decides; nobody does -> HOST. */
 xccl_status_t xccl_mem_component_type(void *ptr, ucs_memory_type_t *mem_type)
@@ -425,6 +527,7 @@ void xccl_mem_component_finalize(void)
             void *handle       = mem_components[mt]->dlhandle;
             mem_components[mt] = NULL;
             mem_extensions[mt] = NULL;
+            mem_steps[mt]      = NULL;
             dlclose(handle);
         }
     }

@@ -35,6 +35,7 @@
 #include "xccl_rocm_mem_component.h"
 #include "xccl_rocm_mem_pool.h"
 #include "mc_pool.h"
+#include "step_plan.h"
 
 #include <hip/hip_runtime_api.h>
 #include <pthread.h>
@@ -768,6 +769,78 @@ static xccl_status_t mc_rocm_do_reduce_multi(void *sbuf1, void *sbuf2,
         }
     }
     return st;
+}
+
+/* The entries of mc_step.c: kernels that have no completion word of their own,
+ * so an event is a recorded HIP event and a blocking call waits for the
+ * stream.  Ordered against the calling thread's reductions as those are among
+ * themselves. */
+xccl_status_t mc_rocm_enqueue(xccl_status_t (*launch)(void *arg, void *hip_stream), void *arg, xccl_stream_t *stream,
+                              xccl_mc_event_t **event, int want_sync)
+{
+    mc_rocm_event_t   done = {.direct = 0, .slot = -1};
+    mc_rocm_event_t  *ev   = NULL;
+    mc_rocm_device_t *d;
+    hipStream_t       hs;
+    xccl_status_t     st;
+
+    if (stream != NULL) {
+        st = mc_rocm_user_stream(stream, &hs);
+        if (st != XCCL_OK) {
+            return st;
+        }
+        st = mc_rocm_device_for_stream(&d, hs);
+    } else {
+        st = mc_rocm_device(&d);
+        if (st == XCCL_OK) {
+            st = mc_rocm_thread_stream(d, &hs);
+        }
+    }
+    if (st != XCCL_OK) {
+        return st;
+    }
+    if (event != NULL) {
+        ev = mc_rocm_claim_event(d);
+        if (ev == NULL) {
+            return XCCL_ERR_NO_RESOURCE;
+        }
+    }
+    if (stream == NULL) {
+        done.slot = mc_rocm_thread_slot();
+        mc_rocm_wait_last_direct();
+    }
+    st = launch(arg, hs);
+    if (stream == NULL) {
+        /* counted even if it failed: part of it may be in the stream */
+        done.stream_seq = atomic_fetch_add_explicit(&d->stream_issued[done.slot], 1, memory_order_acq_rel) + 1;
+    }
+    done.dev = d;
+    if (st == XCCL_OK && want_sync) {
+        if (hipStreamSynchronize(hs) != hipSuccess) {
+            st = XCCL_ERR_NO_MESSAGE;
+        } else {
+            mc_rocm_note_complete(&done);
+        }
+    }
+    if (ev == NULL) {
+        return st;
+    }
+    ev->flagged    = 0;
+    ev->direct     = 0;
+    ev->stream     = hs;
+    ev->slot       = done.slot;
+    ev->stream_seq = done.stream_seq;
+    ev->dev        = d;
+    if (st == XCCL_OK && hipEventRecord(ev->hip_event, hs) != hipSuccess) {
+        st = XCCL_ERR_NO_MESSAGE;
+    }
+    if (st != XCCL_OK) {
+        atomic_store(&ev->is_free, MC_SLOT_FREE);
+        return st;
+    }
+    ev->super.mem_type = UCS_MEMORY_TYPE_ROCM;
+    *event             = &ev->super;
+    return XCCL_OK;
 }
 
 static xccl_status_t mc_rocm_reduce(void *sbuf1, void *sbuf2, void *target,

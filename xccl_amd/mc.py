@@ -1,5 +1,5 @@
 """ctypes mirror of the mem-component boundary (include/xccl_rocm_mem_component.h,
-include/xccl_rocm_kernels.h).
+include/xccl_rocm_kernels.h, include/xccl_rocm_step.h).
 
 Function names, argument order and status codes are those of the reference
 dispatcher (src/utils/mem_component.h:52-95); every function returns the
@@ -61,6 +61,50 @@ class RocmMemComponent(_c.Structure):
                                          _c.POINTER(_vp))),
         ("event_wait", _c.CFUNCTYPE(_ST, _vp)),
         ("get_stream", _c.CFUNCTYPE(_ST, _c.POINTER(_vp))),
+    ]
+
+
+# ---- optimizer step (include/xccl_rocm_step.h) ----
+
+STEP_BLOCK = 256        # XCCL_ROCM_STEP_BLOCK
+STEP_MAX_PEERS = 255    # XCCL_ROCM_STEP_MAX_PEERS
+
+
+class StepLayout(_c.Structure):
+    """xccl_rocm_step_layout_t"""
+    _fields_ = [("grad_dtype", _int), ("param_dtype", _int), ("copy_dtype", _int), ("state_bits", _c.c_uint32),
+                ("n_peers", _c.c_uint32), ("peer_stride", _sz)]
+
+
+class StepTensor(_c.Structure):
+    """xccl_rocm_step_tensor_t"""
+    _fields_ = [("grad", _vp), ("peers", _vp), ("folded", _vp), ("param", _vp), ("copy", _vp), ("exp_avg", _vp),
+                ("exp_avg_sq", _vp), ("exp_avg_scale", _vp), ("exp_avg_sq_scale", _vp), ("size", _sz),
+                ("weight_decay", _c.c_double)]
+
+
+class StepClock(_c.Structure):
+    """xccl_rocm_step_clock_t (lives in device memory)"""
+    _fields_ = [("lr", _c.c_double), ("steps", _c.c_uint64)]
+
+
+class AdamwArgs(_c.Structure):
+    """xccl_rocm_adamw_args_t; `stats` and `clock` are device addresses or None"""
+    _fields_ = [("lr", _c.c_double), ("beta1", _c.c_double), ("beta2", _c.c_double), ("eps", _c.c_double),
+                ("grad_scale", _c.c_double), ("max_norm", _c.c_double), ("step", _c.c_uint64), ("stats", _vp),
+                ("clock", _vp), ("use_folded", _int)]
+
+
+class RocmStepComponent(_c.Structure):
+    """xccl_rocm_step_component_t"""
+    _fields_ = [
+        ("version", _c.c_uint32),
+        ("plan_create", _c.CFUNCTYPE(_ST, _c.POINTER(StepLayout), _c.POINTER(StepTensor), _sz, _c.POINTER(_vp))),
+        ("plan_destroy", _c.CFUNCTYPE(_ST, _vp)),
+        ("grad_norm", _c.CFUNCTYPE(_ST, _vp, _vp)),
+        ("grad_norm_nb", _c.CFUNCTYPE(_ST, _vp, _vp, _c.POINTER(XcclStream), _c.POINTER(_vp))),
+        ("adamw", _c.CFUNCTYPE(_ST, _vp, _c.POINTER(AdamwArgs))),
+        ("adamw_nb", _c.CFUNCTYPE(_ST, _vp, _c.POINTER(AdamwArgs), _c.POINTER(XcclStream), _c.POINTER(_vp))),
     ]
 
 
@@ -153,6 +197,13 @@ def bind_dispatcher(path, mode=_c.DEFAULT_MODE):
                                          _c.POINTER(_vp)],
         "xccl_mem_component_reduce_multi_nb": [_vp, _vp, _vp, _sz, _sz, _sz, _int, _int, _int,
                                                _c.POINTER(XcclStream), _c.POINTER(_vp)],
+        "xccl_mem_component_step_plan_create": [_c.POINTER(StepLayout), _c.POINTER(StepTensor), _sz, _int,
+                                                _c.POINTER(_vp)],
+        "xccl_mem_component_step_plan_destroy": [_vp, _int],
+        "xccl_mem_component_grad_norm": [_vp, _vp, _int],
+        "xccl_mem_component_grad_norm_nb": [_vp, _vp, _int, _c.POINTER(XcclStream), _c.POINTER(_vp)],
+        "xccl_mem_component_adamw": [_vp, _c.POINTER(AdamwArgs), _int],
+        "xccl_mem_component_adamw_nb": [_vp, _c.POINTER(AdamwArgs), _int, _c.POINTER(XcclStream), _c.POINTER(_vp)],
         "xccl_mem_component_memcpy_async": [_vp, _vp, _sz, _c.POINTER(XcclStream)],
         "xccl_mem_component_start_acitivity": [_c.POINTER(XcclStream), _c.POINTER(_vp)],
         "xccl_mem_component_finish_acitivity": [_vp],
@@ -317,6 +368,70 @@ def xccl_mem_component_free_cache():
 
 def xccl_mem_component_finalize():
     dispatch_lib().xccl_mem_component_finalize()
+
+
+# ---- optimizer step (include/xccl_rocm_step.h) ----
+
+def xccl_mem_component_step_plan_create(layout: StepLayout, tensors, mem_type):
+    """`tensors`: a sequence of StepTensor; returns (Status, plan or None)."""
+    plan = _vp()
+    table = (StepTensor * max(len(tensors), 1))(*tensors)
+    st = dispatch_lib().xccl_mem_component_step_plan_create(_c.byref(layout), table, len(tensors), int(mem_type),
+                                                            _c.byref(plan))
+    return _st(st), plan.value
+
+
+def xccl_mem_component_step_plan_destroy(plan, mem_type) -> Status:
+    return _st(dispatch_lib().xccl_mem_component_step_plan_destroy(plan, int(mem_type)))
+
+
+def xccl_mem_component_grad_norm(plan, stats, mem_type) -> Status:
+    return _st(dispatch_lib().xccl_mem_component_grad_norm(plan, stats, int(mem_type)))
+
+
+def xccl_mem_component_grad_norm_nb(plan, stats, mem_type, stream=None, want_event=True):
+    ev = _vp()
+    st = dispatch_lib().xccl_mem_component_grad_norm_nb(plan, stats, int(mem_type), stream.ref() if stream else None,
+                                                        _c.byref(ev) if want_event else None)
+    return _st(st), ev.value
+
+
+def xccl_mem_component_adamw(plan, args: AdamwArgs, mem_type) -> Status:
+    return _st(dispatch_lib().xccl_mem_component_adamw(plan, _c.byref(args), int(mem_type)))
+
+
+def xccl_mem_component_adamw_nb(plan, args: AdamwArgs, mem_type, stream=None, want_event=True):
+    ev = _vp()
+    st = dispatch_lib().xccl_mem_component_adamw_nb(plan, _c.byref(args), int(mem_type),
+                                                    stream.ref() if stream else None,
+                                                    _c.byref(ev) if want_event else None)
+    return _st(st), ev.value
+
+
+class StepPlan:
+    """Owns a plan of the ROCm component; destroyed on close() / garbage collection."""
+
+    def __init__(self, layout: StepLayout, tensors, mem_type=MemType.ROCM):
+        self.mem_type = mem_type
+        st, self.handle = xccl_mem_component_step_plan_create(layout, tensors, mem_type)
+        if st != Status.OK:
+            raise RuntimeError("xccl_mem_component_step_plan_create: %s" % st)
+
+    def close(self):
+        if self.handle:
+            xccl_mem_component_step_plan_destroy(self.handle, self.mem_type)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def step_component() -> RocmStepComponent:
+    """The object behind `xccl_rocm_mem_component_step`."""
+    return _c.POINTER(RocmStepComponent).in_dll(component_lib(), "xccl_rocm_mem_component_step").contents
 
 
 def component_stream():

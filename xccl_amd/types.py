@@ -58,6 +58,10 @@ class Dt(enum.IntEnum):
     UNSUPPORTED = 14
 
 
+# XCCL_ROCM_DT_BFLOAT16 (include/xccl_rocm_step.h): a type of the optimizer step's entries only, not a member of xccl_dt_t
+BFLOAT16 = 15
+
+
 class MemType(enum.IntEnum):
     """ucs_memory_type_t of UCX v1.10."""
     HOST = 0
