@@ -197,10 +197,50 @@ static size_t step_up(size_t n)
     return (n + 255) & ~(size_t)255;
 }
 
+/* A wave's stores that begin and end inside 128-byte lines leave two lines
+ * half written, and its loads touch one line more.  Chunks are moved by up to
+ * 63 elements so that as many of the arrays as possible, by bytes touched, have
+ * them on lines: all of them where the tensors are slices of flat buffers at
+ * the same place.  Blocks of 8-bit states begin with the tensor and cannot move.
+ * Measured, step in 32 bits on 32 Mi elements, all arrays 4 bytes off their
+ * lines: 137 us on lines, 174-218 us as they lie. */
+static uint32_t step_shift(const xccl_rocm_step_layout_t *l, const xccl_rocm_step_tensor_t *t)
+{
+    const struct {
+        const void *ptr;
+        size_t      elem;
+        unsigned    times;
+    } arrays[] = {
+        {t->grad, step_dt_size(l->grad_dtype), 1},   {t->peers, step_dt_size(l->grad_dtype), l->n_peers},
+        {t->folded, step_dt_size(l->grad_dtype), 2}, {t->param, step_dt_size(l->param_dtype), 3},
+        {t->copy, 2, 2},                             {t->exp_avg, 4, 3},
+        {t->exp_avg_sq, 4, 3},
+    };
+    uint32_t shift, best = 0;
+    size_t   score, most = 0, k;
+
+    if (l->state_bits == 8) {
+        return 0;
+    }
+    for (shift = 0; shift < 64; shift++) {
+        for (score = 0, k = 0; k < sizeof(arrays) / sizeof(arrays[0]); k++) {
+            /* chunk 1 begins at element STEP_CHUNK - shift */
+            if (arrays[k].ptr != NULL && ((uintptr_t)arrays[k].ptr + (STEP_CHUNK - shift) * arrays[k].elem) % 128 == 0) {
+                score += arrays[k].times * arrays[k].elem;
+            }
+        }
+        if (score > most) {
+            most = score;
+            best = shift;
+        }
+    }
+    return best;
+}
+
 /* Lays the tables out in host memory, and on the device in one allocation. */
 static xccl_status_t step_build(xccl_rocm_step_plan_t *plan, const xccl_rocm_step_tensor_t *tensors, size_t count)
 {
-    size_t        i, entries = 0, chunks = 0, bytes, at_chunks, at_partials, at_arrivals;
+    size_t        i, entries = 0, chunks = 0, bytes, at_chunks, at_partials, at_arrivals, at_scalars;
     uint32_t      k;
     char         *image;
     step_entry_t *e;
@@ -209,18 +249,21 @@ static xccl_status_t step_build(xccl_rocm_step_plan_t *plan, const xccl_rocm_ste
     xccl_status_t st;
 
     for (i = 0; i < count; i++) {
-        entries += tensors[i].size != 0;
-        chunks += (tensors[i].size + STEP_CHUNK - 1) / STEP_CHUNK;
+        if (tensors[i].size != 0) {
+            entries++;
+            chunks += (tensors[i].size + step_shift(&plan->layout, &tensors[i]) + STEP_CHUNK - 1) / STEP_CHUNK;
+        }
     }
-    if (chunks > 0x7fffffffu) { /* one workgroup each */
+    if (chunks > STEP_MAX_CHUNKS) {
         fprintf(stderr, "xccl mc_rocm: step plan: %zu pieces of %u elements, at most %u are possible\n", chunks,
-                STEP_CHUNK, 0x7fffffffu);
+                STEP_CHUNK, STEP_MAX_CHUNKS);
         return XCCL_ERR_INVALID_PARAM;
     }
     at_chunks   = step_up(entries * sizeof(*e));
     at_partials = at_chunks + step_up(chunks * sizeof(*c));
-    at_arrivals = at_partials + STEP_NORM_GRID * sizeof(step_partial_t);
-    bytes       = at_arrivals + 256;
+    at_arrivals = at_partials + STEP_FOLD_GRID * sizeof(step_partial_t);
+    at_scalars  = at_arrivals + step_up(STEP_ARRIVAL_BYTES);
+    bytes       = at_scalars + 256;
     image       = (char *)calloc(1, bytes);
     if (image == NULL) {
         return XCCL_ERR_NO_MEMORY;
@@ -237,9 +280,9 @@ static xccl_status_t step_build(xccl_rocm_step_plan_t *plan, const xccl_rocm_ste
             .grad = (const char *)t->grad, .peers = (const char *)t->peers, .folded = (char *)t->folded,
             .param = (char *)t->param, .copy = (char *)t->copy, .avg = (char *)t->exp_avg,
             .sq = (char *)t->exp_avg_sq, .avg_scale = t->exp_avg_scale, .sq_scale = t->exp_avg_sq_scale,
-            .size = t->size, .decay = t->weight_decay,
+            .size = t->size, .decay = t->weight_decay, .shift = step_shift(&plan->layout, t),
         };
-        for (k = 0; k < (t->size + STEP_CHUNK - 1) / STEP_CHUNK; k++) {
+        for (k = 0; k < (t->size + e[entries].shift + STEP_CHUNK - 1) / STEP_CHUNK; k++) {
             *c++ = (step_chunk_t){.entry = (uint32_t)entries, .index = k};
         }
         entries++;
@@ -263,6 +306,7 @@ static xccl_status_t step_build(xccl_rocm_step_plan_t *plan, const xccl_rocm_ste
     plan->chunk_table = (step_chunk_t *)(plan->memory + at_chunks);
     plan->partials    = (step_partial_t *)(plan->memory + at_partials);
     plan->arrivals    = (uint32_t *)(plan->memory + at_arrivals);
+    plan->scalars     = (step_scalars_t *)(plan->memory + at_scalars);
     return st;
 }
 

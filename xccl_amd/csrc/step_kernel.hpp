@@ -3,131 +3,217 @@
 // states.  Formulas: include/xccl_rocm_step.h.
 //
 // Both stream: nothing is read twice and nothing but registers lies between
-// load and store.  The unit of work is a chunk, STEP_CHUNK consecutive
-// elements of one tensor, found through the plan's chunk table; a wave takes
-// tiles of 256 elements, 4 consecutive ones per lane, so that a 32-bit array
-// moves as one 16-byte access per lane and an 8-bit block (256 elements of a
-// tensor) is exactly one tile: its maximum is a reduction within the wave.
-// Vector accesses are emitted whatever the alignment (the device runs in
-// unaligned access mode); the last tile of a tensor goes element by element
-// where a lane's four are not all there.
+// load and store.  Elements are found through the plan's table of chunks,
+// STEP_CHUNK consecutive elements of one tensor each.  Accesses are buffer
+// instructions as in reduce_kernel.hpp: the base sits in scalar registers, the
+// alignment may be any (the device runs in unaligned access mode), what lies
+// beyond the descriptor's length is read as zero and not written.  That length
+// is honoured per 32-bit word, so the last elements of a tensor of 8- or 16-bit
+// values go one by one.
 #pragma once
 
 #include "step_plan.h"
 
 #include <hip/hip_runtime.h>
 
+// Pointers that come out of memory are generic to the compiler; this says that
+// they are not, where a plain access goes through one.
+#define STEP_GLOBAL __attribute__((address_space(1)))
+
 namespace xccl_rocm {
 
-constexpr uint32_t kStepThreads = 256;
-constexpr uint32_t kStepWaves   = kStepThreads / 64;
-constexpr uint32_t kStepTile    = 256; // elements a wave takes at once
-constexpr uint32_t kStepTiles   = STEP_CHUNK / kStepTile;
-static_assert(kStepTile == XCCL_ROCM_STEP_BLOCK, "a tile is a block of the 8-bit states");
+typedef float    f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4s __attribute__((ext_vector_type(4)));
 
-typedef float f32x4 __attribute__((ext_vector_type(4)));
+// Cache policy: loads nt, stores sc0 sc1 (written through).
+constexpr int kStepAuxLoad  = 0x02;
+constexpr int kStepAuxStore = 0x11;
 
-// The entries' pointers come out of memory; without the address space the
-// compiler would have to use flat accesses for them.
-#define STEP_GLOBAL __attribute__((address_space(1)))
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t step_rsrc(const char *base, uint32_t bytes)
+{
+    return __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, (int)bytes, 0x00027000);
+}
 
 // ---- four consecutive elements, as 32-bit numbers -------------------------
 
-template <typename T> struct Four {
-    typedef T V __attribute__((ext_vector_type(4)));
-    typedef V VU __attribute__((aligned(sizeof(T)))); // wherever an element may lie
-    static __device__ __forceinline__ f32x4 load(const char *p, uint64_t e)
+template <typename T, int Bytes = sizeof(T)> struct Four;
+
+template <typename T> struct Four<T, 4> {
+    static __device__ __forceinline__ f32x4 load(__amdgpu_buffer_rsrc_t r, uint32_t off)
     {
-        return __builtin_convertvector((V)__builtin_nontemporal_load((const STEP_GLOBAL VU *)((const T *)p + e)), f32x4);
+        return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, kStepAuxLoad));
     }
-    static __device__ __forceinline__ void store(char *p, uint64_t e, f32x4 x)
+    static __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t r, uint32_t off, f32x4 x)
     {
-        __builtin_nontemporal_store((VU)__builtin_convertvector(x, V), (STEP_GLOBAL VU *)((T *)p + e));
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4s, x), r, (int)off, 0, kStepAuxStore);
     }
 };
 
-// `count` of a lane's four elements exist (uniformly 4 but for a tensor's last tile).
-template <typename T>
-__device__ __forceinline__ f32x4 load4(const char *p, uint64_t e, uint32_t count)
-{
-    if (count == 4) {
-        return Four<T>::load(p, e);
+template <typename T> struct Four<T, 2> {
+    typedef T V __attribute__((ext_vector_type(4)));
+    static __device__ __forceinline__ f32x4 load(__amdgpu_buffer_rsrc_t r, uint32_t off)
+    {
+        return __builtin_convertvector(
+            __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b64(r, (int)off, 0, kStepAuxLoad)), f32x4);
     }
-    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    static __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t r, uint32_t off, f32x4 x)
+    {
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, __builtin_convertvector(x, V)), r, (int)off, 0,
+                                              kStepAuxStore);
+    }
+};
+
+// One element.
+template <typename T> __device__ __forceinline__ float load_one(__amdgpu_buffer_rsrc_t r, uint32_t off)
+{
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, (int)off, 0, kStepAuxLoad));
+    } else {
+        return (float)__builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(r, (int)off, 0, kStepAuxLoad));
+    }
+}
+
+template <typename T> __device__ __forceinline__ void store_one(__amdgpu_buffer_rsrc_t r, uint32_t off, float x)
+{
+    if constexpr (sizeof(T) == 4) {
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, x), r, (int)off, 0, kStepAuxStore);
+    } else {
+        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, (T)x), r, (int)off, 0, kStepAuxStore);
+    }
+}
+
+// Up to 256 consecutive elements of a tensor, 4 to a lane.  Full: all 256.
+struct Span {
+    uint64_t first;
+    uint32_t left;
+};
+
+// Tile `i` of a tensor: its elements in [256 i - shift, 256 (i + 1) - shift).
+__device__ __forceinline__ Span tile_span(const step_entry_t &t, uint64_t i)
+{
+    const int64_t from = (int64_t)(i * 256) - t.shift;
+    const int64_t to   = from + 256 < (int64_t)t.size ? from + 256 : (int64_t)t.size;
+    Span          s;
+    s.first = from < 0 ? 0 : (uint64_t)from;
+    s.left  = to > (int64_t)s.first ? (uint32_t)(to - (int64_t)s.first) : 0;
+    return s;
+}
+
+template <typename T, bool Full>
+__device__ __forceinline__ f32x4 load4(const char *p, const Span &s, uint32_t lane)
+{
+    const __amdgpu_buffer_rsrc_t r   = step_rsrc(p + s.first * sizeof(T), s.left * (uint32_t)sizeof(T));
+    const uint32_t               off = lane * 4 * (uint32_t)sizeof(T);
+    if (Full || sizeof(T) == 4) {
+        return Four<T>::load(r, off);
+    }
+    f32x4 x;
 #pragma unroll
-    for (uint32_t k = 0; k < 3; ++k) {
-        if (k < count) {
-            x[k] = (float)((const STEP_GLOBAL T *)p)[e + k];
-        }
+    for (uint32_t k = 0; k < 4; ++k) {
+        x[k] = load_one<T>(r, off + k * (uint32_t)sizeof(T));
     }
     return x;
 }
 
-template <typename T>
-__device__ __forceinline__ void store4(char *p, uint64_t e, uint32_t count, f32x4 x)
+template <typename T, bool Full>
+__device__ __forceinline__ void store4(char *p, const Span &s, uint32_t lane, f32x4 x)
 {
-    if (count == 4) {
-        Four<T>::store(p, e, x);
+    const __amdgpu_buffer_rsrc_t r   = step_rsrc(p + s.first * sizeof(T), s.left * (uint32_t)sizeof(T));
+    const uint32_t               off = lane * 4 * (uint32_t)sizeof(T);
+    if (Full || sizeof(T) == 4) {
+        Four<T>::store(r, off, x);
         return;
     }
 #pragma unroll
-    for (uint32_t k = 0; k < 3; ++k) {
-        if (k < count) {
-            ((STEP_GLOBAL T *)p)[e + k] = (T)x[k];
-        }
+    for (uint32_t k = 0; k < 4; ++k) {
+        store_one<T>(r, off + k * (uint32_t)sizeof(T), x[k]);
     }
 }
 
-__device__ __forceinline__ uint32_t load_codes(const char *p, uint64_t e, uint32_t count)
+template <bool Full> __device__ __forceinline__ uint32_t load_codes(const char *p, const Span &s, uint32_t lane)
 {
-    typedef uint32_t U __attribute__((aligned(1)));
-    if (count == 4) {
-        return __builtin_nontemporal_load((const STEP_GLOBAL U *)(p + e));
+    const __amdgpu_buffer_rsrc_t r = step_rsrc(p + s.first, s.left);
+    if (Full) {
+        return __builtin_amdgcn_raw_buffer_load_b32(r, (int)lane * 4, 0, kStepAuxLoad);
     }
     uint32_t x = 0;
 #pragma unroll
-    for (uint32_t k = 0; k < 3; ++k) {
-        if (k < count) {
-            x |= (uint32_t)((const STEP_GLOBAL uint8_t *)p)[e + k] << (8 * k);
-        }
+    for (uint32_t k = 0; k < 4; ++k) {
+        x |= (uint32_t)__builtin_amdgcn_raw_buffer_load_b8(r, (int)(lane * 4 + k), 0, kStepAuxLoad) << (8 * k);
     }
     return x;
 }
 
-__device__ __forceinline__ void store_codes(char *p, uint64_t e, uint32_t count, uint32_t x)
+template <bool Full>
+__device__ __forceinline__ void store_codes(char *p, const Span &s, uint32_t lane, uint32_t x)
 {
-    typedef uint32_t U __attribute__((aligned(1)));
-    if (count == 4) {
-        __builtin_nontemporal_store(x, (STEP_GLOBAL U *)(p + e));
+    const __amdgpu_buffer_rsrc_t r = step_rsrc(p + s.first, s.left);
+    if (Full) {
+        __builtin_amdgcn_raw_buffer_store_b32(x, r, (int)lane * 4, 0, kStepAuxStore);
         return;
     }
 #pragma unroll
-    for (uint32_t k = 0; k < 3; ++k) {
-        if (k < count) {
-            ((STEP_GLOBAL uint8_t *)p)[e + k] = (uint8_t)(x >> (8 * k));
+    for (uint32_t k = 0; k < 4; ++k) {
+        __builtin_amdgcn_raw_buffer_store_b8((uint8_t)(x >> (8 * k)), r, (int)(lane * 4 + k), 0, kStepAuxStore);
+    }
+}
+
+// a = grad + peer{0}; a = peer{j} + a: reduce_multi's order, in 32 bits whatever
+// the gradient's type, N tiles at once.  As there the vectors are walked one by
+// one with two in flight; the last of them is requested by begin and added by
+// end, so that the caller can request what else it needs in between.
+template <typename G, bool Full, bool Peers, int N> struct Fold {
+    f32x4 sum[N], more[Peers ? N : 1];
+
+    static __device__ __forceinline__ void request(f32x4 *to, const char *p, const Span *s, uint32_t lane)
+    {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            to[i] = load4<G, Full>(p, s[i], lane);
         }
     }
-}
 
-// Elements of the lane's four that exist, for the tile whose first element is e0.
-__device__ __forceinline__ uint32_t lane_count(uint64_t size, uint64_t e)
-{
-    return e >= size ? 0u : (size - e < 4 ? (uint32_t)(size - e) : 4u);
-}
-
-// a = grad + peer{0}; a = peer{j} + a: reduce_multi's order, in 32 bits whatever the gradient's type.
-template <typename G>
-__device__ __forceinline__ f32x4 fold4(const char *grad, const char *peers, uint32_t n_peers, size_t stride, uint64_t e,
-                                       uint32_t count)
-{
-    f32x4 a = load4<G>(grad, e, count);
-    for (uint32_t j = 0; j < n_peers; ++j) {
-        a = load4<G>(peers + j * stride, e, count) + a;
+    __device__ __forceinline__ void add(const f32x4 *x)
+    {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            sum[i] = x[i] + sum[i];
+        }
     }
-    return a;
-}
+
+    __device__ __forceinline__ void begin(const char *grad, const char *peers, uint32_t n_peers, size_t stride,
+                                          const Span *s, uint32_t lane)
+    {
+        request(sum, grad, s, lane);
+        if constexpr (Peers) {
+            request(more, peers, s, lane);
+            for (uint32_t j = 1; j < n_peers; ++j) {
+                f32x4 next[N];
+                peers += stride;
+                request(next, peers, s, lane);
+                __builtin_amdgcn_sched_barrier(0);
+                add(more);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    more[i] = next[i];
+                }
+            }
+        }
+    }
+
+    __device__ __forceinline__ void end()
+    {
+        if constexpr (Peers) {
+            add(more);
+        }
+    }
+};
 
 // ---- the norm ---------------------------------------------------------------
+
+constexpr uint32_t kNormWaves = 4; // of a workgroup
 
 struct NormArgs {
     const step_entry_t *entries;
@@ -142,128 +228,283 @@ struct NormArgs {
     uint32_t            writes_fold;
 };
 
-__device__ __forceinline__ double wave_sum(double x)
-{
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-        x += __shfl_xor(x, d);
-    }
-    return x;
-}
+// What a thread, a wave, a workgroup has found.
+struct NormTotal {
+    double   sum;
+    uint64_t bad;
 
-// Sum over the workgroup, in thread 0.
-__device__ __forceinline__ double group_sum(double x, double *lds)
-{
-    x = wave_sum(x);
-    if ((threadIdx.x & 63) == 0) {
-        lds[threadIdx.x >> 6] = x;
-    }
-    __syncthreads();
-    x = 0;
-    for (uint32_t w = 0; w < kStepWaves; ++w) {
-        x += lds[w];
-    }
-    __syncthreads();
-    return x;
-}
-
-// Which chunks a workgroup takes and the order of every sum depend on the plan
-// alone, so equal gradients give equal results.  The squares are summed in 64
-// bits: a 32-bit square would overflow from 1.8e19 and vanish below 1e-23.
-// The last workgroup to arrive adds the partial results up.
-template <typename G>
-__global__ void __launch_bounds__(kStepThreads) grad_norm_kernel(const NormArgs a)
-{
-    __shared__ double lds[kStepWaves];
-    __shared__ bool   last;
-    const uint32_t    lane = threadIdx.x & 63;
-    const uint32_t    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    double            sum  = 0;
-    uint32_t          bad  = 0;
-
-    for (uint32_t c = blockIdx.x; c < a.n_chunks; c += a.grid) {
-        const step_chunk_t chunk = a.chunks[c];
-        const step_entry_t t     = a.entries[chunk.entry];
-        const uint64_t     first = (uint64_t)chunk.index * STEP_CHUNK;
-        for (uint32_t i = wave; i < kStepTiles; i += kStepWaves) {
-            const uint64_t tile = first + i * kStepTile;
-            if (tile >= t.size) {
-                break;
-            }
-            const uint64_t e     = tile + lane * 4;
-            const uint32_t count = lane_count(t.size, e);
-            f32x4          x     = fold4<G>(t.grad, t.peers, a.n_peers, a.peer_stride, e, count);
-            if (a.n_peers != 0) {
-                // rounded to the gradient's type, written or not: the norm does not depend on whether it is
+    // Over the workgroup, in every thread.
+    __device__ __forceinline__ void gather(NormTotal *lds)
+    {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    x[k] = (float)(G)x[k];
-                }
-                if (a.writes_fold) {
-                    store4<G>(t.folded, e, count, x);
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const double d = (double)x[k];
-                sum = __builtin_fma(d, d, sum);
-                bad += !__builtin_isfinite(x[k]);
-            }
+        for (int d = 32; d > 0; d >>= 1) {
+            sum += __shfl_xor(sum, d);
+            bad += __shfl_xor(bad, d);
         }
+        if ((threadIdx.x & 63) == 0) {
+            lds[threadIdx.x >> 6] = *this;
+        }
+        __syncthreads();
+        sum = lds[0].sum;
+        bad = lds[0].bad;
+#pragma unroll
+        for (uint32_t w = 1; w < kNormWaves; ++w) {
+            sum += lds[w].sum;
+            bad += lds[w].bad;
+        }
+        __syncthreads();
     }
-    sum             = group_sum(sum, lds);
-    double bad_sum = group_sum((double)bad, lds);
+};
+
+// What the threads have found -> stats.  The last workgroup to arrive adds the
+// partial results up, in an order that does not depend on who that is.
+__device__ __forceinline__ void norm_finish(const NormArgs &a, NormTotal t)
+{
+    __shared__ NormTotal lds[kNormWaves];
+    __shared__ bool      last;
+    t.gather(lds);
     if (a.grid > 1) {
         if (threadIdx.x == 0) {
             // written through to memory, and there before this workgroup counts itself in
-            __hip_atomic_store(&a.partials[blockIdx.x].sum, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-            __hip_atomic_store(&a.partials[blockIdx.x].bad, bad_sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+            __hip_atomic_store(&a.partials[blockIdx.x].sum, t.sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+            __hip_atomic_store(&a.partials[blockIdx.x].bad, t.bad, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            last = atomicInc(a.arrivals, a.grid - 1) == a.grid - 1; // wraps to 0: ready for the next launch
+            // in two levels: arrivals on one counter take their turn, 12 ns each
+            const uint32_t shards = a.grid < STEP_ARRIVAL_SHARDS ? a.grid : STEP_ARRIVAL_SHARDS;
+            const uint32_t shard  = blockIdx.x % shards;
+            const uint32_t total  = a.grid / shards + (shard < a.grid % shards ? 1u : 0u);
+            bool           end    = atomicInc(a.arrivals + (1 + shard) * STEP_ARRIVAL_STRIDE, total - 1) == total - 1;
+            if (end) { // (atomicInc wraps to 0 at its bound: ready for the next launch)
+                end = atomicInc(a.arrivals, shards - 1) == shards - 1;
+            }
+            last = end;
         }
         __syncthreads();
         if (!last) {
             return;
         }
-        sum     = 0;
-        bad_sum = 0;
-        for (uint32_t b = threadIdx.x; b < a.grid; b += kStepThreads) {
-            sum += __hip_atomic_load(&a.partials[b].sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
-            bad_sum += __hip_atomic_load(&a.partials[b].bad, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+        t = {0, 0};
+        for (uint32_t b = threadIdx.x; b < a.grid; b += kNormWaves * 64) {
+            t.sum += __hip_atomic_load(&a.partials[b].sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
+            t.bad += __hip_atomic_load(&a.partials[b].bad, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
         }
-        sum     = group_sum(sum, lds);
-        bad_sum = group_sum(bad_sum, lds);
+        t.gather(lds);
     }
     if (threadIdx.x == 0) {
-        a.stats[0] = sum;
-        a.stats[1] = bad_sum;
+        a.stats[0] = t.sum;
+        a.stats[1] = (double)t.bad;
     }
+}
+
+// Squares are summed in 64 bits: in 32 they would overflow from 1.8e19 and
+// vanish below 1e-23.  Two chains of additions, one for each half of the lane's elements.
+struct NormSum {
+    double   even = 0, odd = 0;
+    uint32_t bad = 0;
+    __device__ __forceinline__ void add(float x, bool is_odd)
+    {
+        const double d = (double)x;
+        double      &s = is_odd ? odd : even;
+        s              = __builtin_fma(d, d, s);
+        bad += !__builtin_isfinite(x);
+    }
+    __device__ __forceinline__ NormTotal total() const
+    {
+        return {even + odd, bad};
+    }
+};
+
+// The elements of one chunk: 16 bytes per lane and load.
+template <typename G> struct NormChunk {
+    static constexpr int Loads = STEP_CHUNK * sizeof(G) / 1024;
+    u32x4s               x[Loads];
+    uint16_t             last; // 16-bit types: the odd element behind the whole words
+
+    __device__ __forceinline__ void load(const char *base, uint32_t left)
+    {
+        const uint32_t               bytes = left * (uint32_t)sizeof(G);
+        const uint32_t               lane  = threadIdx.x & 63;
+        const __amdgpu_buffer_rsrc_t r     = step_rsrc(base, bytes & ~3u);
+#pragma unroll
+        for (int i = 0; i < Loads; ++i) {
+            x[i] = __builtin_amdgcn_raw_buffer_load_b128(r, (int)(i * 1024 + lane * 16), 0, kStepAuxLoad);
+        }
+        if constexpr (sizeof(G) == 2) {
+            last = __builtin_amdgcn_raw_buffer_load_b16(step_rsrc(base + (bytes & ~3u), bytes & 3u), (int)lane * 2, 0, kStepAuxLoad);
+        }
+    }
+
+    __device__ __forceinline__ void sum(NormSum &s) const
+    {
+        typedef G V __attribute__((ext_vector_type(16 / sizeof(G))));
+#pragma unroll
+        for (int i = 0; i < Loads; ++i) {
+            const V v = __builtin_bit_cast(V, x[i]);
+#pragma unroll
+            for (uint32_t k = 0; k < 16 / sizeof(G); ++k) {
+                s.add((float)v[k], k & 1);
+            }
+        }
+        if constexpr (sizeof(G) == 2) {
+            s.add((float)__builtin_bit_cast(G, last), false);
+        }
+    }
+};
+
+struct Piece {
+    const char *base;
+    uint32_t    left; // elements; 0 behind the last chunk
+};
+
+__device__ __forceinline__ step_chunk_t norm_chunk(const NormArgs &a, uint32_t c)
+{
+    return a.chunks[c < a.n_chunks ? c : a.n_chunks - 1];
+}
+
+__device__ __forceinline__ Piece norm_piece(const NormArgs &a, uint32_t c, step_chunk_t chunk, uint32_t elem)
+{
+    const step_entry_t *t    = a.entries + chunk.entry;
+    const int64_t       from = (int64_t)chunk.index * STEP_CHUNK - t->shift;
+    const int64_t       to   = from + STEP_CHUNK < (int64_t)t->size ? from + STEP_CHUNK : (int64_t)t->size;
+    const int64_t       at   = from < 0 ? 0 : from;
+    Piece               p;
+    p.base = t->grad + at * elem;
+    p.left = c < a.n_chunks ? (uint32_t)(to - at) : 0u;
+    return p;
+}
+
+// One vector per tensor.  Which chunks a wave takes and the order of every sum
+// depend on the plan alone, so equal gradients give equal results.  A wave
+// requests 4 KiB before it sums up the last 4 KiB, has read the tensor's entry
+// for that a round before, and the table's a round before that: no address is
+// waited for.
+template <typename G>
+__global__ void __launch_bounds__(kNormWaves * 64) grad_norm_kernel(const NormArgs a)
+{
+    constexpr uint32_t K    = 4096 / (STEP_CHUNK * sizeof(G)); // chunks at once
+    const uint32_t     wave = blockIdx.x * kNormWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t     step = a.grid * kNormWaves * K;
+    NormSum            s;
+    if (a.n_chunks != 0) {
+        NormChunk<G> x[K], y[K];
+        Piece        piece[K];
+        step_chunk_t chunk[K];
+        uint32_t     c = wave * K; // what x holds; piece is `step` further, chunk `2 * step`
+#pragma unroll
+        for (uint32_t k = 0; k < K; ++k) {
+            piece[k] = norm_piece(a, c + k, norm_chunk(a, c + k), sizeof(G));
+            chunk[k] = norm_chunk(a, c + step + k);
+        }
+        auto advance = [&](NormChunk<G>(&to)[K], uint32_t at) {
+#pragma unroll
+            for (uint32_t k = 0; k < K; ++k) {
+                to[k].load(piece[k].base, piece[k].left);
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < K; ++k) {
+                piece[k] = norm_piece(a, at + step + k, chunk[k], sizeof(G));
+                chunk[k] = norm_chunk(a, at + 2 * step + k);
+            }
+        };
+        auto sum = [&](const NormChunk<G>(&of)[K]) {
+#pragma unroll
+            for (uint32_t k = 0; k < K; ++k) {
+                of[k].sum(s);
+            }
+        };
+        advance(x, c);
+        while (c < a.n_chunks) {
+            advance(y, c + step);
+            sum(x);
+            advance(x, c + 2 * step);
+            sum(y);
+            c += 2 * step;
+        }
+    }
+    norm_finish(a, s.total());
+}
+
+// With peers' vectors: a wave folds N tiles at a time, and writes the fold if
+// there is a place for it.
+constexpr int      kFoldTiles   = 2;
+constexpr uint32_t kFoldPerChunk = STEP_CHUNK / 256 / kFoldTiles;
+
+template <typename G, bool Full, int N>
+__device__ __forceinline__ void fold_tiles(const NormArgs &a, const step_entry_t &t, const Span *span, NormSum &s)
+{
+    const uint32_t           lane = threadIdx.x & 63;
+    Fold<G, Full, true, N>   fold;
+    fold.begin(t.grad, t.peers, a.n_peers, a.peer_stride, span, lane);
+    fold.end();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        f32x4 x = fold.sum[i];
+        // rounded to the gradient's type, written or not: the norm does not depend on whether it is
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            x[k] = (float)(G)x[k];
+            s.add(x[k], k & 1);
+        }
+        if (a.writes_fold) {
+            store4<G, Full>(t.folded, span[i], lane, x);
+        }
+    }
+}
+
+// Measured, 3 peers, 16 Mi elements, 32 bits, the fold written (335 MB): tiles at
+// once 1 / 2 / 4 with 512 workgroups 98 / 65 / 65 us, 1024: 64 / 57 / 60, 2048:
+// 59 / 59 / 59, 4096: 61 / 60 / 60.
+template <typename G>
+__global__ void __launch_bounds__(kNormWaves * 64) fold_norm_kernel(const NormArgs a)
+{
+    constexpr int  N    = kFoldTiles;
+    const uint32_t wave = blockIdx.x * kNormWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    NormSum        s;
+    for (uint32_t u = wave; u < a.n_chunks * kFoldPerChunk; u += a.grid * kNormWaves) {
+        const step_chunk_t chunk = a.chunks[u / kFoldPerChunk];
+        const step_entry_t t     = a.entries[chunk.entry];
+        const uint64_t     first = (uint64_t)chunk.index * (STEP_CHUNK / 256) + u % kFoldPerChunk * N;
+        Span               span[N];
+        uint32_t           have = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            span[i] = tile_span(t, first + i);
+            have += span[i].left;
+        }
+        if (have == 256 * N) {
+            fold_tiles<G, true, N>(a, t, span, s);
+        } else {
+            for (int i = 0; i < N; ++i) {
+                const Span one = tile_span(t, first + i);
+                fold_tiles<G, false, 1>(a, t, &one, s);
+            }
+        }
+    }
+    norm_finish(a, s.total());
 }
 
 // ---- AdamW ------------------------------------------------------------------
 
+// A workgroup is one wave and takes one tile: 256 consecutive elements of a
+// tensor, 4 to a lane.  A 32-bit array moves as one 16-byte access per lane, and
+// an 8-bit block is exactly one tile: its maximum is a reduction within the wave.
+constexpr uint32_t kStepTile  = 256;
+constexpr uint32_t kStepTiles = STEP_CHUNK / kStepTile;
+static_assert(kStepTile == XCCL_ROCM_STEP_BLOCK, "a tile is a block of the 8-bit states");
+
 struct AdamwKernelArgs {
-    const step_entry_t           *entries;
-    const step_chunk_t           *chunks;
-    const double                 *stats;
-    const xccl_rocm_step_clock_t *clock;
-    size_t                        peer_stride;
-    uint32_t                      n_peers;
-    uint32_t                      use_folded;
-    uint32_t                      copy; // 0 none, 1 FLOAT16, 2 BFLOAT16
-    float                         b1, omb1, b2, omb2, eps;
-    double                        beta1, beta2, lr, grad_scale, max_norm;
-    uint64_t                      step;
+    const step_entry_t   *entries;
+    const step_chunk_t   *chunks;
+    const step_scalars_t *from; // device: read instead of `s` if not NULL
+    step_scalars_t        s;
+    size_t                peer_stride;
+    uint32_t              n_peers;
+    uint32_t              use_folded;
+    uint32_t              copy; // 0 none, 1 FLOAT16, 2 BFLOAT16
+    float                 b1, omb1, b2, omb2, eps;
 };
 
-// What depends on step number, rate and norm; 64 bits, because 1 - beta^t loses its digits in 32 for small t.
-struct StepScalars {
-    double lr;
-    float  g;      // factor of the folded gradient
-    float  size;   // lr / (1 - beta1^t)
-    float  inv_c2; // 1 / sqrt(1 - beta2^t)
-};
-
+// base^n; the relative error grows with n, to n 2^-53, where base^n itself vanishes.
 __host__ __device__ inline double power(double base, uint64_t n)
 {
     double x = 1;
@@ -276,39 +517,80 @@ __host__ __device__ inline double power(double base, uint64_t n)
     return x;
 }
 
-__device__ __forceinline__ StepScalars step_scalars(const AdamwKernelArgs &a)
+// 64 bits, because 1 - beta^t loses its digits in 32 for small t.
+__host__ __device__ inline void step_rate(step_scalars_t &s, double beta1, double beta2, double lr, uint64_t t)
 {
-    const uint64_t t  = a.clock ? a.clock->steps + 1 : a.step;
-    const double   lr = a.clock ? a.clock->lr : a.lr;
-    double         k  = a.grad_scale;
+    s.lr     = lr;
+    s.size   = (float)(lr / (1 - power(beta1, t)));
+    s.inv_c2 = (float)(1 / sqrt(1 - power(beta2, t)));
+}
+
+// Ahead of the step, where step number, rate or norm come from device memory;
+// counts the step unless it is skipped.
+struct ScalarArgs {
+    step_scalars_t         *to;
+    const double           *stats;
+    xccl_rocm_step_clock_t *clock;
+    double                  beta1, beta2, lr, grad_scale, max_norm;
+    uint64_t                step;
+};
+
+__global__ void step_scalars_kernel(const ScalarArgs a)
+{
+    step_scalars_t s;
+    s.skip   = a.stats != nullptr && !(a.stats[1] == 0);
+    double k = a.grad_scale;
     if (a.max_norm > 0) {
         const double clip = a.max_norm / (sqrt(a.stats[0]) * a.grad_scale + 1e-6);
         k *= clip < 1 ? clip : 1;
     }
-    StepScalars s;
-    s.lr     = lr;
-    s.g      = (float)k;
-    s.size   = (float)(lr / (1 - power(a.beta1, t)));
-    s.inv_c2 = (float)(1 / sqrt(1 - power(a.beta2, t)));
-    return s;
+    s.g              = (float)k;
+    const uint64_t t = a.clock ? a.clock->steps + 1 : a.step;
+    step_rate(s, a.beta1, a.beta2, a.clock ? a.clock->lr : a.lr, t);
+    *a.to = s;
+    if (a.clock && !s.skip) {
+        a.clock->steps = t;
+    }
+}
+
+// Maximum over the wave, in a scalar register: within rows of 16 lanes (shifts
+// by 1, 2, 4, 8), then from row to row; lane 63 ends up with all of it.
+template <int Ctrl, int Rows> __device__ __forceinline__ uint32_t max_step(uint32_t x)
+{
+    const uint32_t y = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, Ctrl, Rows, 0xf, false);
+    return y > x ? y : x;
 }
 
 __device__ __forceinline__ uint32_t wave_max(uint32_t x)
 {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-        const uint32_t y = __shfl_xor(x, d);
-        x = y > x ? y : x;
-    }
-    return x;
+    x = max_step<0x111, 0xf>(x);
+    x = max_step<0x112, 0xf>(x);
+    x = max_step<0x114, 0xf>(x);
+    x = max_step<0x118, 0xf>(x);
+    x = max_step<0x142, 0xa>(x); // row 0's last lane to row 1, row 2's to row 3
+    x = max_step<0x143, 0xc>(x); // row 1's last lane to rows 2 and 3
+    return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
+}
+
+// The correctly rounded square root: the hardware's is off by one unit of the
+// last place at most, and which of the three is nearest tells the sign of what
+// the product with a neighbour leaves of x (Tuckerman's test).  Below 2^-125
+// those remainders vanish and the hardware's result stays; 0 and infinity do too.
+__device__ __forceinline__ float nearest_sqrt(float x)
+{
+    const float    s     = __builtin_amdgcn_sqrtf(x);
+    const uint32_t bits  = __builtin_bit_cast(uint32_t, s);
+    const float    below = __builtin_bit_cast(float, bits - 1), above = __builtin_bit_cast(float, bits + 1);
+    float          r     = __builtin_fmaf(-below, s, x) <= 0 ? below : s;
+    return __builtin_fmaf(-above, s, x) > 0 ? above : r;
 }
 
 // Four e4m3 codes of x, and the power of two they are to be multiplied with.
 // Magnitudes order as their bits do; adding 0x1fffff carries into the exponent
 // iff the mantissa is above 1.75, i.e. iff 448 of 2^(exponent - 8) is too small.
-// Positive: what is above zero stays above zero.
+// Positive: where `of`, the square of x, is above zero the code is too.
 template <bool Positive>
-__device__ __forceinline__ uint32_t quantize(f32x4 x, float &scale)
+__device__ __forceinline__ uint32_t quantize(f32x4 x, f32x4 of, float &scale)
 {
     uint32_t most = 0;
 #pragma unroll
@@ -327,7 +609,7 @@ __device__ __forceinline__ uint32_t quantize(f32x4 x, float &scale)
     for (int k = 0; k < 4; ++k) {
         y[k] = x[k] * inv;
         if (Positive) {
-            y[k] = x[k] > 0 && y[k] < 0x1p-9f ? 0x1p-9f : y[k];
+            y[k] = of[k] > 0 && y[k] < 0x1p-9f ? 0x1p-9f : y[k];
         }
     }
     int code = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
@@ -341,72 +623,89 @@ __device__ __forceinline__ f32x4 dequantize(uint32_t codes, float scale)
     return f32x4{lo[0] * scale, lo[1] * scale, hi[0] * scale, hi[1] * scale};
 }
 
-template <typename P, typename G, bool Eight>
-__global__ void __launch_bounds__(kStepThreads) adamw_kernel(const AdamwKernelArgs a)
+template <typename P, typename G, bool Eight, bool Peers, bool Full>
+__device__ __forceinline__ void adamw_tile(const AdamwKernelArgs &a, const step_scalars_t &s, const step_entry_t &t,
+                                           const Span &span)
 {
-    if (a.stats != nullptr && a.stats[1] != 0) {
-        return; // a gradient that is not finite: the whole step is skipped
+    const uint32_t          lane  = threadIdx.x;
+    const uint64_t          block = span.first / kStepTile;
+    f32x4                   m, v, r;
+    uint32_t                m_codes, r_codes;
+    float                   m_scale, r_scale;
+    Fold<G, Full, Peers, 1> fold;
+    fold.begin(a.use_folded ? t.folded : t.grad, t.peers, a.n_peers, a.peer_stride, &span, lane);
+    f32x4 p = load4<P, Full>(t.param, span, lane);
+    if constexpr (Eight) {
+        m_codes = load_codes<Full>(t.avg, span, lane);
+        r_codes = load_codes<Full>(t.sq, span, lane);
+        m_scale = ((const STEP_GLOBAL float *)t.avg_scale)[block];
+        r_scale = ((const STEP_GLOBAL float *)t.sq_scale)[block];
+    } else {
+        m = load4<float, Full>(t.avg, span, lane);
+        v = load4<float, Full>(t.sq, span, lane);
     }
-    const StepScalars  s     = step_scalars(a);
-    const step_chunk_t chunk = a.chunks[blockIdx.x];
-    const step_entry_t t     = a.entries[chunk.entry];
-    const uint64_t     first = (uint64_t)chunk.index * STEP_CHUNK;
-    const uint32_t     lane  = threadIdx.x & 63;
-    const uint32_t     wave  = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const float        keep  = (float)(1 - s.lr * t.decay);
-    const char        *grad  = a.use_folded ? t.folded : t.grad;
-
-    for (uint32_t i = wave; i < kStepTiles; i += kStepWaves) {
-        const uint64_t tile = first + i * kStepTile;
-        if (tile >= t.size) {
-            break;
-        }
-        const uint64_t e     = tile + lane * 4;
-        const uint32_t count = lane_count(t.size, e);
-        const f32x4    g     = fold4<G>(grad, t.peers, a.n_peers, a.peer_stride, e, count) * s.g;
-        f32x4          p     = load4<P>(t.param, e, count);
-        f32x4          m, v, r;
-        if (Eight) {
-            m = dequantize(load_codes(t.avg, e, count), ((STEP_GLOBAL float *)t.avg_scale)[tile / kStepTile]);
-            r = dequantize(load_codes(t.sq, e, count), ((STEP_GLOBAL float *)t.sq_scale)[tile / kStepTile]);
-            v = r * r;
-        } else {
-            m = load4<float>(t.avg, e, count);
-            v = load4<float>(t.sq, e, count);
-        }
-        m = m * a.b1 + g * a.omb1;
-        v = v * a.b2 + (g * a.omb2) * g;
+    const float keep = (float)(1 - s.lr * t.decay);
+    fold.end();
+    const f32x4 g = fold.sum[0] * s.g;
+    if constexpr (Eight) {
+        m = dequantize(m_codes, m_scale);
+        r = dequantize(r_codes, r_scale);
+        v = r * r;
+    }
+    m = m * a.b1 + g * a.omb1;
+    v = v * a.b2 + (g * a.omb2) * g;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            r[k] = sqrtf(v[k]);
-            p[k] = p[k] * keep - s.size * (m[k] / (r[k] * s.inv_c2 + a.eps));
+    for (int k = 0; k < 4; ++k) {
+        const float vk = v[k];
+        // The hardware's square root and reciprocal are within one unit of the last place, two roundings of the many
+        // that the parameter sees.  The square root that is stored as a code is the correctly rounded one: a block's
+        // scale hangs on it.
+        r[k] = Eight ? nearest_sqrt(vk) : __builtin_amdgcn_sqrtf(vk);
+        p[k] = p[k] * keep - s.size * (m[k] * __builtin_amdgcn_rcpf(r[k] * s.inv_c2 + a.eps));
+    }
+    store4<P, Full>(t.param, span, lane, p);
+    if (a.copy == 1) {
+        store4<_Float16, Full>(t.copy, span, lane, p);
+    } else if (a.copy == 2) {
+        store4<__bf16, Full>(t.copy, span, lane, p);
+    }
+    if constexpr (Eight) {
+        store_codes<Full>(t.avg, span, lane, quantize<false>(m, m, m_scale));
+        store_codes<Full>(t.sq, span, lane, quantize<true>(r, v, r_scale));
+        if (lane == 0) {
+            ((STEP_GLOBAL float *)t.avg_scale)[block] = m_scale;
+            ((STEP_GLOBAL float *)t.sq_scale)[block]  = r_scale;
         }
-        store4<P>(t.param, e, count, p);
-        if (a.copy == 1) {
-            store4<_Float16>(t.copy, e, count, p);
-        } else if (a.copy == 2) {
-            store4<__bf16>(t.copy, e, count, p);
-        }
-        if (Eight) {
-            float m_scale, r_scale;
-            store_codes(t.avg, e, count, quantize<false>(m, m_scale));
-            store_codes(t.sq, e, count, quantize<true>(r, r_scale));
-            if (lane == 0) {
-                ((STEP_GLOBAL float *)t.avg_scale)[tile / kStepTile] = m_scale;
-                ((STEP_GLOBAL float *)t.sq_scale)[tile / kStepTile]  = r_scale;
-            }
-        } else {
-            store4<float>(t.avg, e, count, m);
-            store4<float>(t.sq, e, count, v);
-        }
+    } else {
+        store4<float, Full>(t.avg, span, lane, m);
+        store4<float, Full>(t.sq, span, lane, v);
     }
 }
 
-// Behind the step, which reads the number: counts it, unless it was skipped.
-__global__ void clock_kernel(xccl_rocm_step_clock_t *clock, const double *stats)
+template <typename P, typename G, bool Eight, bool Peers>
+__global__ void __launch_bounds__(64) adamw_kernel(const AdamwKernelArgs a)
 {
-    if (stats == nullptr || stats[1] == 0) {
-        clock->steps += 1;
+    // Both lie in memory that is constant meanwhile: a choice of addresses, and no branch in front of the loads below.
+    typedef const __attribute__((address_space(4))) char           *Constant;
+    typedef const __attribute__((address_space(4))) step_scalars_t *Scalars;
+    const Constant given = (Constant)__builtin_amdgcn_kernarg_segment_ptr() + offsetof(AdamwKernelArgs, s);
+    const Scalars  from  = (Scalars)(a.from != nullptr ? (Constant)a.from : given);
+    step_scalars_t s;
+    s.lr     = from->lr;
+    s.g      = from->g;
+    s.size   = from->size;
+    s.inv_c2 = from->inv_c2;
+    s.skip   = from->skip;
+    const step_chunk_t chunk = a.chunks[blockIdx.x / kStepTiles];
+    const step_entry_t t     = a.entries[chunk.entry];
+    Span               span  = tile_span(t, (uint64_t)chunk.index * kStepTiles + blockIdx.x % kStepTiles);
+    if (s.skip) {
+        span.left = 0; // a gradient that is not finite: nothing is read or written
+    }
+    if (span.left == kStepTile) {
+        adamw_tile<P, G, Eight, Peers, true>(a, s, t, span);
+    } else if (span.left != 0) {
+        adamw_tile<P, G, Eight, Peers, false>(a, s, t, span);
     }
 }
 

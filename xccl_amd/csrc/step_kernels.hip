@@ -1,7 +1,9 @@
 // step_kernels.hip -- launches of the optimizer step's kernels (step_kernel.hpp).
 #include "step_kernel.hpp"
 
+#include <math.h>
 #include <stdio.h>
+#include <string.h>
 
 using namespace xccl_rocm;
 
@@ -19,24 +21,58 @@ xccl_status_t launched(const char *what)
 
 typedef void (*AdamwKernel)(AdamwKernelArgs);
 
-template <typename P, bool Eight>
-AdamwKernel adamw_by_grad(xccl_dt_t grad)
+template <typename P, typename G>
+AdamwKernel adamw_by_form(bool eight, bool peers)
+{
+    return eight ? (peers ? adamw_kernel<P, G, true, true> : adamw_kernel<P, G, true, false>)
+                 : (peers ? adamw_kernel<P, G, false, true> : adamw_kernel<P, G, false, false>);
+}
+
+template <typename P>
+AdamwKernel adamw_by_grad(xccl_dt_t grad, bool eight, bool peers)
 {
     switch ((int)grad) {
-    case XCCL_DT_FLOAT32: return adamw_kernel<P, float, Eight>;
-    case XCCL_DT_FLOAT16: return adamw_kernel<P, _Float16, Eight>;
-    default:              return adamw_kernel<P, __bf16, Eight>;
+    case XCCL_DT_FLOAT32: return adamw_by_form<P, float>(eight, peers);
+    case XCCL_DT_FLOAT16: return adamw_by_form<P, _Float16>(eight, peers);
+    default:              return adamw_by_form<P, __bf16>(eight, peers);
     }
 }
 
-template <bool Eight>
-AdamwKernel adamw_by_types(xccl_dt_t param, xccl_dt_t grad)
+AdamwKernel adamw_by_types(xccl_dt_t param, xccl_dt_t grad, bool eight, bool peers)
 {
     switch ((int)param) {
-    case XCCL_DT_FLOAT32: return adamw_by_grad<float, Eight>(grad);
-    case XCCL_DT_FLOAT16: return adamw_by_grad<_Float16, Eight>(grad);
-    default:              return adamw_by_grad<__bf16, Eight>(grad);
+    case XCCL_DT_FLOAT32: return adamw_by_grad<float>(grad, eight, peers);
+    case XCCL_DT_FLOAT16: return adamw_by_grad<_Float16>(grad, eight, peers);
+    default:              return adamw_by_grad<__bf16>(grad, eight, peers);
     }
+}
+
+// LDS that a workgroup (one wave) of the step asks for and never touches, to
+// bound how many share a compute unit: as many as keep 54 KiB of loads in
+// flight, one gradient vector counted (56 KiB with 8-bit states, which take
+// longer from load to store).  More of them only disturb each other's order of
+// access to memory; a step that mostly stays in the memory-side cache does not mind.  Measured, us at 0 / 6 / 7 / 8 / 10 / 12 / 16 KiB asked for (32 /
+// 26 / 22 / 20 / 16 / 13 / 10 waves):
+//   32-bit states, all 32 bits, 256 Mi elements   1188 1207 1177 1146 1135 1115 1161
+//   32-bit states, bf16 gradient and copy, 64 Mi   310  309  303  299  297  304  325
+//   32-bit states, 3 peers, bf16 copy, 32 Mi       238  236  231  229  227  213  225
+//   8-bit states, 32-bit gradient, 256 Mi          712  675  643  665  695  816  996
+//   8-bit states, bf16 gradient and copy, 64 Mi    175  174  182  194  202  237  284
+//   8-bit states, bf16, 1 peer, 24 Mi (200 MB)      52   56   62   68   74   90  113
+//   32-bit states, fp16, 8 Mi (100 MB)              34   34   34   35   35   37   40
+unsigned adamw_lds(const xccl_rocm_step_plan_t *plan, uint32_t n_peers)
+{
+    const xccl_rocm_step_layout_t &l       = plan->layout;
+    const unsigned                 grad    = l.grad_dtype == XCCL_DT_FLOAT32 ? 4 : 2;
+    const unsigned                 param   = l.param_dtype == XCCL_DT_FLOAT32 ? 4 : 2;
+    const unsigned                 states  = l.state_bits == 8 ? 2 : 8;
+    const unsigned                 loads   = (grad + param + states) * kStepTile;
+    const unsigned                 waves   = (l.state_bits == 8 ? 56 : 54) * 1024 / loads;
+    const size_t                   touched = plan->chunks * STEP_CHUNK * ((1 + n_peers) * grad + param + states);
+    if (waves >= 32 || touched <= (size_t)192 << 20) {
+        return 0;
+    }
+    return 160 * 1024 / waves & ~511u;
 }
 
 } // namespace
@@ -45,7 +81,8 @@ extern "C" {
 
 xccl_status_t step_launch_grad_norm(const xccl_rocm_step_plan_t *plan, double *stats, void *hip_stream)
 {
-    NormArgs a;
+    const bool fold = plan->layout.n_peers != 0;
+    NormArgs   a;
     a.entries     = plan->entries;
     a.chunks      = plan->chunk_table;
     a.partials    = plan->partials;
@@ -55,18 +92,22 @@ xccl_status_t step_launch_grad_norm(const xccl_rocm_step_plan_t *plan, double *s
     a.n_chunks    = (uint32_t)plan->chunks;
     a.n_peers     = plan->layout.n_peers;
     a.writes_fold = plan->writes_fold;
-    a.grid        = a.n_chunks < 1 ? 1 : a.n_chunks < STEP_NORM_GRID ? a.n_chunks : STEP_NORM_GRID;
-    const dim3        grid(a.grid), block(kStepThreads);
+    // one wave for each unit of work, up to a grid that is resident at once and then goes round
+    const uint32_t units = fold ? a.n_chunks * kFoldPerChunk : a.n_chunks;
+    const uint32_t want  = (units + kNormWaves - 1) / kNormWaves;
+    const uint32_t most  = fold ? STEP_FOLD_GRID : STEP_NORM_GRID;
+    a.grid               = want < 1 ? 1 : want < most ? want : most;
+    const dim3        grid(a.grid), block(kNormWaves * 64);
     const hipStream_t s = (hipStream_t)hip_stream;
     switch ((int)plan->layout.grad_dtype) {
     case XCCL_DT_FLOAT32:
-        hipLaunchKernelGGL(grad_norm_kernel<float>, grid, block, 0, s, a);
+        hipLaunchKernelGGL(fold ? fold_norm_kernel<float> : grad_norm_kernel<float>, grid, block, 0, s, a);
         break;
     case XCCL_DT_FLOAT16:
-        hipLaunchKernelGGL(grad_norm_kernel<_Float16>, grid, block, 0, s, a);
+        hipLaunchKernelGGL(fold ? fold_norm_kernel<_Float16> : grad_norm_kernel<_Float16>, grid, block, 0, s, a);
         break;
     default:
-        hipLaunchKernelGGL(grad_norm_kernel<__bf16>, grid, block, 0, s, a);
+        hipLaunchKernelGGL(fold ? fold_norm_kernel<__bf16> : grad_norm_kernel<__bf16>, grid, block, 0, s, a);
         break;
     }
     return launched("grad_norm");
@@ -75,11 +116,12 @@ xccl_status_t step_launch_grad_norm(const xccl_rocm_step_plan_t *plan, double *s
 xccl_status_t step_launch_adamw(const xccl_rocm_step_plan_t *plan, const xccl_rocm_adamw_args_t *args, void *hip_stream)
 {
     const xccl_rocm_step_layout_t &l = plan->layout;
-    AdamwKernelArgs a;
+    const hipStream_t              s = (hipStream_t)hip_stream;
+    AdamwKernelArgs                a;
     a.entries     = plan->entries;
     a.chunks      = plan->chunk_table;
-    a.stats       = args->stats;
-    a.clock       = args->clock;
+    a.from        = nullptr;
+    a.s.skip      = 0;
     a.peer_stride = l.peer_stride;
     a.n_peers     = args->use_folded ? 0 : l.n_peers;
     a.use_folded  = args->use_folded != 0;
@@ -89,28 +131,34 @@ xccl_status_t step_launch_adamw(const xccl_rocm_step_plan_t *plan, const xccl_ro
     a.b2          = (float)args->beta2;
     a.omb2        = (float)(1 - args->beta2);
     a.eps         = (float)args->eps;
-    a.beta1       = args->beta1;
-    a.beta2       = args->beta2;
-    a.lr          = args->lr;
-    a.grad_scale  = args->grad_scale;
-    a.max_norm    = args->max_norm;
-    a.step        = args->step;
-
-    const hipStream_t s = (hipStream_t)hip_stream;
-    if (plan->chunks != 0) {
-        const AdamwKernel k = l.state_bits == 8 ? adamw_by_types<true>(l.param_dtype, l.grad_dtype)
-                                                : adamw_by_types<false>(l.param_dtype, l.grad_dtype);
-        hipLaunchKernelGGL(k, dim3((unsigned)plan->chunks), dim3(kStepThreads), 0, s, a);
-        const xccl_status_t st = launched("adamw");
+    a.s.g         = (float)args->grad_scale;
+    if (args->clock != nullptr || args->stats != nullptr) {
+        ScalarArgs c;
+        c.to         = plan->scalars;
+        c.stats      = args->stats;
+        c.clock      = args->clock;
+        c.beta1      = args->beta1;
+        c.beta2      = args->beta2;
+        c.lr         = args->lr;
+        c.grad_scale = args->grad_scale;
+        c.max_norm   = args->max_norm;
+        c.step       = args->step;
+        hipLaunchKernelGGL(step_scalars_kernel, dim3(1), dim3(1), 0, s, c);
+        const xccl_status_t st = launched("the step's scalars");
         if (st != XCCL_OK) {
             return st;
         }
+        a.from = plan->scalars;
+        memset(&a.s, 0, sizeof(a.s));
+    } else {
+        step_rate(a.s, args->beta1, args->beta2, args->lr, args->step);
     }
-    if (args->clock != nullptr) {
-        hipLaunchKernelGGL(clock_kernel, dim3(1), dim3(1), 0, s, args->clock, args->stats);
-        return launched("the step clock");
+    if (plan->chunks == 0) {
+        return XCCL_OK;
     }
-    return XCCL_OK;
+    const AdamwKernel k = adamw_by_types(l.param_dtype, l.grad_dtype, l.state_bits == 8, a.n_peers != 0);
+    hipLaunchKernelGGL(k, dim3((unsigned)plan->chunks * kStepTiles), dim3(64), adamw_lds(plan, a.n_peers), s, a);
+    return launched("adamw");
 }
 
 } // extern "C"

@@ -12,7 +12,9 @@
 extern "C" {
 #endif
 
-/* One non-empty tensor, as the kernels read it. */
+/* One non-empty tensor, as the kernels read it.  `shift`: elements by which its
+ * chunks are moved towards its start, so that they begin on cache lines of as
+ * much of what the kernels touch as possible. */
 typedef struct step_entry {
     const char *grad;
     const char *peers;
@@ -25,32 +27,50 @@ typedef struct step_entry {
     float      *sq_scale;
     uint64_t    size;
     double      decay;
+    uint32_t    shift;
 } step_entry_t;
 
-/* STEP_CHUNK consecutive elements of a tensor (fewer at its end): a workgroup's unit of work. */
-#define STEP_CHUNK 4096u
+/* Chunk i of a tensor: those of its elements that lie in [i * STEP_CHUNK - shift, (i + 1) * STEP_CHUNK - shift). */
+#define STEP_CHUNK 1024u
 typedef struct step_chunk {
     uint32_t entry;
     uint32_t index;
 } step_chunk_t;
+#define STEP_MAX_CHUNKS 0x1fffffffu /* a step launches four workgroups for each */
 
-/* grad_norm runs at most this many workgroups; each leaves one partial result. */
-#define STEP_NORM_GRID 2048u
+/* grad_norm runs at most this many workgroups, without and with peers; each leaves one partial result. */
+#define STEP_NORM_GRID 512u
+#define STEP_FOLD_GRID 1024u
 typedef struct step_partial {
-    double sum;
-    double bad;
+    double   sum;
+    uint64_t bad;
 } step_partial_t;
+
+/* Arrivals are counted in two levels, one counter per 128-byte line: STEP_ARRIVAL_SHARDS of them behind the last one. */
+#define STEP_ARRIVAL_SHARDS 64u
+#define STEP_ARRIVAL_STRIDE 32u
+#define STEP_ARRIVAL_BYTES ((1 + STEP_ARRIVAL_SHARDS) * STEP_ARRIVAL_STRIDE * 4)
+
+/* What depends on step number, rate and norm. */
+typedef struct step_scalars {
+    double   lr;
+    float    g;      /* factor of the folded gradient */
+    float    size;   /* lr / (1 - beta1^t) */
+    float    inv_c2; /* 1 / sqrt(1 - beta2^t) */
+    uint32_t skip;   /* the gradient is not finite */
+} step_scalars_t;
 
 struct xccl_rocm_step_plan {
     xccl_rocm_step_layout_t layout;
     int                     device;
     int                     writes_fold;
     size_t                  chunks;
-    char                   *memory;   /* device: the one allocation behind the four pointers below */
+    char                   *memory;   /* device: the one allocation behind the five pointers below */
     step_entry_t           *entries;
     step_chunk_t           *chunk_table;
-    step_partial_t         *partials; /* STEP_NORM_GRID of them */
-    uint32_t               *arrivals; /* workgroups of grad_norm that are through; zero between launches */
+    step_partial_t         *partials; /* STEP_FOLD_GRID of them */
+    uint32_t               *arrivals; /* workgroups of grad_norm that are through (STEP_ARRIVAL_BYTES); zero between launches */
+    step_scalars_t         *scalars;  /* of the step that runs, where they come from device memory */
 };
 
 #define STEP_INTERNAL __attribute__((visibility("hidden")))

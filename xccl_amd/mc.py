@@ -270,7 +270,7 @@ class Stream:
 
     def __init__(self, hip_stream, stype=StreamType.ROCM):
         self._handle = _vp(hip_stream)
-        self.xccl = XcclStream(int(stype), _c.cast(_c.pointer(self._handle), _vp))
+        self.xccl = XcclStream(int(stype), _c.addressof(self._handle))
 
     @property
     def hip_stream(self):
