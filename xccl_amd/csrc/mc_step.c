@@ -306,6 +306,7 @@ static xccl_status_t step_build(xccl_rocm_step_plan_t *plan, const xccl_rocm_ste
     plan->chunk_table = (step_chunk_t *)(plan->memory + at_chunks);
     plan->partials    = (step_partial_t *)(plan->memory + at_partials);
     plan->arrivals    = (uint32_t *)(plan->memory + at_arrivals);
+    plan->zero        = (double *)(plan->memory + at_scalars + 128);
     plan->scalars     = (step_scalars_t *)(plan->memory + at_scalars);
     return st;
 }

@@ -26,9 +26,13 @@ typedef float    f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4s __attribute__((ext_vector_type(4)));
 
-// Cache policy: loads nt, stores sc0 sc1 (written through).
-constexpr int kStepAuxLoad  = 0x02;
-constexpr int kStepAuxStore = 0x11;
+// Cache policy: loads nt; stores written through (sc0 sc1) or nt.  With 32-bit
+// gradients writing through is faster, with 16-bit ones nt is.  Measured, step,
+// written through / nt, us: 32-bit gradients, 32-bit states 256 Mi 1112 / 1135, 3
+// peers 32 Mi 215 / 221, 8-bit states 256 Mi 640 / 658; 16-bit gradients, 32-bit
+// states 64 Mi 299 / 290, 8-bit states 64 Mi 177 / 173, 1 peer 24 Mi 52 / 51.
+constexpr int kStepAuxLoad = 0x02;
+template <typename G> constexpr int kStepAuxStore = sizeof(G) == 4 ? 0x11 : 0x02;
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t step_rsrc(const char *base, uint32_t bytes)
 {
@@ -44,9 +48,9 @@ template <typename T> struct Four<T, 4> {
     {
         return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, kStepAuxLoad));
     }
-    static __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t r, uint32_t off, f32x4 x)
+    template <int Aux> static __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t r, uint32_t off, f32x4 x)
     {
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4s, x), r, (int)off, 0, kStepAuxStore);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4s, x), r, (int)off, 0, Aux);
     }
 };
 
@@ -57,10 +61,9 @@ template <typename T> struct Four<T, 2> {
         return __builtin_convertvector(
             __builtin_bit_cast(V, __builtin_amdgcn_raw_buffer_load_b64(r, (int)off, 0, kStepAuxLoad)), f32x4);
     }
-    static __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t r, uint32_t off, f32x4 x)
+    template <int Aux> static __device__ __forceinline__ void store(__amdgpu_buffer_rsrc_t r, uint32_t off, f32x4 x)
     {
-        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, __builtin_convertvector(x, V)), r, (int)off, 0,
-                                              kStepAuxStore);
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, __builtin_convertvector(x, V)), r, (int)off, 0, Aux);
     }
 };
 
@@ -74,12 +77,12 @@ template <typename T> __device__ __forceinline__ float load_one(__amdgpu_buffer_
     }
 }
 
-template <typename T> __device__ __forceinline__ void store_one(__amdgpu_buffer_rsrc_t r, uint32_t off, float x)
+template <typename T, int Aux> __device__ __forceinline__ void store_one(__amdgpu_buffer_rsrc_t r, uint32_t off, float x)
 {
     if constexpr (sizeof(T) == 4) {
-        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, x), r, (int)off, 0, kStepAuxStore);
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, x), r, (int)off, 0, Aux);
     } else {
-        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, (T)x), r, (int)off, 0, kStepAuxStore);
+        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, (T)x), r, (int)off, 0, Aux);
     }
 }
 
@@ -116,18 +119,18 @@ __device__ __forceinline__ f32x4 load4(const char *p, const Span &s, uint32_t la
     return x;
 }
 
-template <typename T, bool Full>
+template <typename T, bool Full, int Aux>
 __device__ __forceinline__ void store4(char *p, const Span &s, uint32_t lane, f32x4 x)
 {
     const __amdgpu_buffer_rsrc_t r   = step_rsrc(p + s.first * sizeof(T), s.left * (uint32_t)sizeof(T));
     const uint32_t               off = lane * 4 * (uint32_t)sizeof(T);
     if (Full || sizeof(T) == 4) {
-        Four<T>::store(r, off, x);
+        Four<T>::template store<Aux>(r, off, x);
         return;
     }
 #pragma unroll
     for (uint32_t k = 0; k < 4; ++k) {
-        store_one<T>(r, off + k * (uint32_t)sizeof(T), x[k]);
+        store_one<T, Aux>(r, off + k * (uint32_t)sizeof(T), x[k]);
     }
 }
 
@@ -145,17 +148,17 @@ template <bool Full> __device__ __forceinline__ uint32_t load_codes(const char *
     return x;
 }
 
-template <bool Full>
+template <bool Full, int Aux>
 __device__ __forceinline__ void store_codes(char *p, const Span &s, uint32_t lane, uint32_t x)
 {
     const __amdgpu_buffer_rsrc_t r = step_rsrc(p + s.first, s.left);
     if (Full) {
-        __builtin_amdgcn_raw_buffer_store_b32(x, r, (int)lane * 4, 0, kStepAuxStore);
+        __builtin_amdgcn_raw_buffer_store_b32(x, r, (int)lane * 4, 0, Aux);
         return;
     }
 #pragma unroll
     for (uint32_t k = 0; k < 4; ++k) {
-        __builtin_amdgcn_raw_buffer_store_b8((uint8_t)(x >> (8 * k)), r, (int)(lane * 4 + k), 0, kStepAuxStore);
+        __builtin_amdgcn_raw_buffer_store_b8((uint8_t)(x >> (8 * k)), r, (int)(lane * 4 + k), 0, Aux);
     }
 }
 
@@ -446,7 +449,7 @@ __device__ __forceinline__ void fold_tiles(const NormArgs &a, const step_entry_t
             s.add(x[k], k & 1);
         }
         if (a.writes_fold) {
-            store4<G, Full>(t.folded, span[i], lane, x);
+            store4<G, Full, kStepAuxStore<G>>(t.folded, span[i], lane, x);
         }
     }
 }
@@ -495,8 +498,13 @@ static_assert(kStepTile == XCCL_ROCM_STEP_BLOCK, "a tile is a block of the 8-bit
 struct AdamwKernelArgs {
     const step_entry_t   *entries;
     const step_chunk_t   *chunks;
-    const step_scalars_t *from; // device: read instead of `s` if not NULL
+    const step_scalars_t *from;  // device: read instead of `s` if not NULL
+    const double         *stats; // device, or NULL
     step_scalars_t        s;
+    double                zero;  // read instead of stats[1] if there is no stats
+    double                grad_scale, max_norm;
+    float                 g;     // factor of the folded gradient, where it is not clipped
+    uint32_t              clip;
     size_t                peer_stride;
     uint32_t              n_peers;
     uint32_t              use_folded;
@@ -525,30 +533,25 @@ __host__ __device__ inline void step_rate(step_scalars_t &s, double beta1, doubl
     s.inv_c2 = (float)(1 / sqrt(1 - power(beta2, t)));
 }
 
-// Ahead of the step, where step number, rate or norm come from device memory;
-// counts the step unless it is skipped.
-struct ScalarArgs {
-    step_scalars_t         *to;
-    const double           *stats;
+// Ahead of a step that has a clock: reads it for the step, and counts the step
+// unless it is going to be skipped.  All loads go out at once, stats[1] from a
+// place that holds 0 if there is none.
+struct ClockArgs {
     xccl_rocm_step_clock_t *clock;
-    double                  beta1, beta2, lr, grad_scale, max_norm;
-    uint64_t                step;
+    const double           *bad;
+    step_scalars_t         *to;
+    double                  beta1, beta2;
 };
 
-__global__ void step_scalars_kernel(const ScalarArgs a)
+__global__ void step_clock_kernel(const ClockArgs a)
 {
+    const double   lr  = a.clock->lr;
+    const uint64_t t   = a.clock->steps + 1;
+    const double   bad = *a.bad;
     step_scalars_t s;
-    s.skip   = a.stats != nullptr && !(a.stats[1] == 0);
-    double k = a.grad_scale;
-    if (a.max_norm > 0) {
-        const double clip = a.max_norm / (sqrt(a.stats[0]) * a.grad_scale + 1e-6);
-        k *= clip < 1 ? clip : 1;
-    }
-    s.g              = (float)k;
-    const uint64_t t = a.clock ? a.clock->steps + 1 : a.step;
-    step_rate(s, a.beta1, a.beta2, a.clock ? a.clock->lr : a.lr, t);
+    step_rate(s, a.beta1, a.beta2, lr, t);
     *a.to = s;
-    if (a.clock && !s.skip) {
+    if (bad == 0) {
         a.clock->steps = t;
     }
 }
@@ -644,9 +647,14 @@ __device__ __forceinline__ void adamw_tile(const AdamwKernelArgs &a, const step_
         m = load4<float, Full>(t.avg, span, lane);
         v = load4<float, Full>(t.sq, span, lane);
     }
-    const float keep = (float)(1 - s.lr * t.decay);
+    const float keep   = (float)(1 - s.lr * t.decay);
+    float       factor = a.g;
+    if (a.clip) {
+        const double k = a.max_norm / (sqrt(*(const __attribute__((address_space(4))) double *)a.stats) * a.grad_scale + 1e-6);
+        factor         = (float)(a.grad_scale * (k < 1 ? k : 1));
+    }
     fold.end();
-    const f32x4 g = fold.sum[0] * s.g;
+    const f32x4 g = fold.sum[0] * factor;
     if constexpr (Eight) {
         m = dequantize(m_codes, m_scale);
         r = dequantize(r_codes, r_scale);
@@ -663,44 +671,44 @@ __device__ __forceinline__ void adamw_tile(const AdamwKernelArgs &a, const step_
         r[k] = Eight ? nearest_sqrt(vk) : __builtin_amdgcn_sqrtf(vk);
         p[k] = p[k] * keep - s.size * (m[k] * __builtin_amdgcn_rcpf(r[k] * s.inv_c2 + a.eps));
     }
-    store4<P, Full>(t.param, span, lane, p);
+    store4<P, Full, kStepAuxStore<G>>(t.param, span, lane, p);
     if (a.copy == 1) {
-        store4<_Float16, Full>(t.copy, span, lane, p);
+        store4<_Float16, Full, kStepAuxStore<G>>(t.copy, span, lane, p);
     } else if (a.copy == 2) {
-        store4<__bf16, Full>(t.copy, span, lane, p);
+        store4<__bf16, Full, kStepAuxStore<G>>(t.copy, span, lane, p);
     }
     if constexpr (Eight) {
-        store_codes<Full>(t.avg, span, lane, quantize<false>(m, m, m_scale));
-        store_codes<Full>(t.sq, span, lane, quantize<true>(r, v, r_scale));
+        store_codes<Full, kStepAuxStore<G>>(t.avg, span, lane, quantize<false>(m, m, m_scale));
+        store_codes<Full, kStepAuxStore<G>>(t.sq, span, lane, quantize<true>(r, v, r_scale));
         if (lane == 0) {
             ((STEP_GLOBAL float *)t.avg_scale)[block] = m_scale;
             ((STEP_GLOBAL float *)t.sq_scale)[block]  = r_scale;
         }
     } else {
-        store4<float, Full>(t.avg, span, lane, m);
-        store4<float, Full>(t.sq, span, lane, v);
+        store4<float, Full, kStepAuxStore<G>>(t.avg, span, lane, m);
+        store4<float, Full, kStepAuxStore<G>>(t.sq, span, lane, v);
     }
 }
 
 template <typename P, typename G, bool Eight, bool Peers>
 __global__ void __launch_bounds__(64) adamw_kernel(const AdamwKernelArgs a)
 {
-    // Both lie in memory that is constant meanwhile: a choice of addresses, and no branch in front of the loads below.
-    typedef const __attribute__((address_space(4))) char           *Constant;
-    typedef const __attribute__((address_space(4))) step_scalars_t *Scalars;
-    const Constant given = (Constant)__builtin_amdgcn_kernarg_segment_ptr() + offsetof(AdamwKernelArgs, s);
-    const Scalars  from  = (Scalars)(a.from != nullptr ? (Constant)a.from : given);
+    // All of it lies in memory that is constant meanwhile: a choice of addresses, and no branch in front of the loads.
+    typedef const __attribute__((address_space(4))) char *Constant;
+    const Constant args = (Constant)__builtin_amdgcn_kernarg_segment_ptr();
+    const auto     from = (const __attribute__((address_space(4))) step_scalars_t *)(
+        a.from != nullptr ? (Constant)a.from : args + offsetof(AdamwKernelArgs, s));
+    const uint64_t bad  = *(const __attribute__((address_space(4))) uint64_t *)(
+        a.stats != nullptr ? (Constant)(a.stats + 1) : args + offsetof(AdamwKernelArgs, zero));
     step_scalars_t s;
     s.lr     = from->lr;
-    s.g      = from->g;
     s.size   = from->size;
     s.inv_c2 = from->inv_c2;
-    s.skip   = from->skip;
     const step_chunk_t chunk = a.chunks[blockIdx.x / kStepTiles];
     const step_entry_t t     = a.entries[chunk.entry];
     Span               span  = tile_span(t, (uint64_t)chunk.index * kStepTiles + blockIdx.x % kStepTiles);
-    if (s.skip) {
-        span.left = 0; // a gradient that is not finite: nothing is read or written
+    if (bad << 1 != 0) {
+        span.left = 0; // not 0 of either sign: a gradient is not finite, nothing is read or written
     }
     if (span.left == kStepTile) {
         adamw_tile<P, G, Eight, Peers, true>(a, s, t, span);

@@ -121,7 +121,12 @@ xccl_status_t step_launch_adamw(const xccl_rocm_step_plan_t *plan, const xccl_ro
     a.entries     = plan->entries;
     a.chunks      = plan->chunk_table;
     a.from        = nullptr;
-    a.s.skip      = 0;
+    a.stats       = args->stats;
+    a.zero        = 0;
+    a.grad_scale  = args->grad_scale;
+    a.max_norm    = args->max_norm;
+    a.g           = (float)args->grad_scale;
+    a.clip        = args->max_norm > 0;
     a.peer_stride = l.peer_stride;
     a.n_peers     = args->use_folded ? 0 : l.n_peers;
     a.use_folded  = args->use_folded != 0;
@@ -131,20 +136,15 @@ xccl_status_t step_launch_adamw(const xccl_rocm_step_plan_t *plan, const xccl_ro
     a.b2          = (float)args->beta2;
     a.omb2        = (float)(1 - args->beta2);
     a.eps         = (float)args->eps;
-    a.s.g         = (float)args->grad_scale;
-    if (args->clock != nullptr || args->stats != nullptr) {
-        ScalarArgs c;
-        c.to         = plan->scalars;
-        c.stats      = args->stats;
-        c.clock      = args->clock;
-        c.beta1      = args->beta1;
-        c.beta2      = args->beta2;
-        c.lr         = args->lr;
-        c.grad_scale = args->grad_scale;
-        c.max_norm   = args->max_norm;
-        c.step       = args->step;
-        hipLaunchKernelGGL(step_scalars_kernel, dim3(1), dim3(1), 0, s, c);
-        const xccl_status_t st = launched("the step's scalars");
+    if (args->clock != nullptr) {
+        ClockArgs c;
+        c.clock = args->clock;
+        c.bad   = args->stats != nullptr ? args->stats + 1 : plan->zero;
+        c.to    = plan->scalars;
+        c.beta1 = args->beta1;
+        c.beta2 = args->beta2;
+        hipLaunchKernelGGL(step_clock_kernel, dim3(1), dim3(1), 0, s, c);
+        const xccl_status_t st = launched("the step's clock");
         if (st != XCCL_OK) {
             return st;
         }

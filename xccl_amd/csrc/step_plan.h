@@ -51,13 +51,11 @@ typedef struct step_partial {
 #define STEP_ARRIVAL_STRIDE 32u
 #define STEP_ARRIVAL_BYTES ((1 + STEP_ARRIVAL_SHARDS) * STEP_ARRIVAL_STRIDE * 4)
 
-/* What depends on step number, rate and norm. */
+/* What depends on step number and rate. */
 typedef struct step_scalars {
-    double   lr;
-    float    g;      /* factor of the folded gradient */
-    float    size;   /* lr / (1 - beta1^t) */
-    float    inv_c2; /* 1 / sqrt(1 - beta2^t) */
-    uint32_t skip;   /* the gradient is not finite */
+    double lr;
+    float  size;   /* lr / (1 - beta1^t) */
+    float  inv_c2; /* 1 / sqrt(1 - beta2^t) */
 } step_scalars_t;
 
 struct xccl_rocm_step_plan {
@@ -65,12 +63,13 @@ struct xccl_rocm_step_plan {
     int                     device;
     int                     writes_fold;
     size_t                  chunks;
-    char                   *memory;   /* device: the one allocation behind the five pointers below */
+    char                   *memory;   /* device: the one allocation behind the pointers below */
     step_entry_t           *entries;
     step_chunk_t           *chunk_table;
     step_partial_t         *partials; /* STEP_FOLD_GRID of them */
     uint32_t               *arrivals; /* workgroups of grad_norm that are through (STEP_ARRIVAL_BYTES); zero between launches */
-    step_scalars_t         *scalars;  /* of the step that runs, where they come from device memory */
+    double                 *zero;     /* holds 0 */
+    step_scalars_t         *scalars;  /* of the step that runs, where there is a clock */
 };
 
 #define STEP_INTERNAL __attribute__((visibility("hidden")))
