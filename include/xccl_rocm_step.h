@@ -22,8 +22,9 @@
  *               - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
  *
  * A whole step is skipped, nothing written and nothing counted, when the
- * `stats` it is given say that an element was not finite: the usual answer to
- * a loss scale that was too large.  Without `stats` such an element goes
+ * `stats` it is given say that an element was not finite (or are no sum of
+ * squares: negative, infinite, NaN): the usual answer to a loss scale that was
+ * too large.  Without `stats` such an element goes
  * through the formulas and poisons its own parameter and states only (its
  * block's states, with states in 8 bits).
  *
@@ -73,7 +74,8 @@ typedef struct xccl_rocm_step_layout {
  * aligned to their element type and to nothing more.  `folded` is where
  * grad_norm writes the folded gradient (rounded once to grad_dtype); given for
  * all tensors or for none, only with peers, and may be exactly `grad` or
- * exactly `peers`.  Apart from that nothing that is written may overlap
+ * exactly `peers`; a step after that reads `folded` (use_folded), since the
+ * vectors it would fold are no longer what they were.  Apart from that nothing that is written may overlap
  * anything else of the plan.  A tensor of size 0 is passed over.
  */
 typedef struct xccl_rocm_step_tensor {
@@ -118,7 +120,13 @@ typedef struct xccl_rocm_step_plan xccl_rocm_step_plan_t;
  * plan_create checks the list (XCCL_ERR_INVALID_PARAM for what the comments
  * above do not allow, XCCL_ERR_UNSUPPORTED for a type without a kernel; says
  * on stderr which tensor), allocates, and synchronises: not inside a capture.
- * The list itself is not kept.  plan_destroy waits for the device.
+ * The list itself is not kept.  plan_destroy waits for the device; graphs that
+ * hold calls on the plan must not run any more.  On the device a plan takes 96
+ * bytes per tensor and 8 (24 without peers) per 1024 elements.
+ *
+ * Steps are fastest when a tensor's arrays begin on 128-byte lines; with states
+ * in 32 bits it is enough that they all begin at the same place of one, as
+ * slices of flat buffers do.
  *
  * grad_norm and adamw are complete on return.  The _nb forms only enqueue, on
  * `stream` or, if that is NULL, on the component's stream of the calling

@@ -233,8 +233,11 @@ def test_skipped_step(bits, value, peers):
         p.arena.download()
         for t in p.tensors:
             assert all(p.arena.unchanged(x) for x in (t.param, t.copy, t.avg, t.sq, t.avg_scale, t.sq_scale) if x is not None)
-        p.set_stats(1.0, np.nan)                                                  # a sum over ranks that went wrong
-        run_step(p, use_stats=True, use_clock=True, use_folded=bool(peers))
+        # sums over ranks that went wrong
+        for wrong in ((1.0, np.nan), (1.0, -1.0), (np.nan, 0.0), (np.inf, 0.0), (-1.0, 0.0)):
+            p.set_stats(*wrong)
+            run_step(p, max_norm=1.0, use_stats=True, use_clock=True, use_folded=bool(peers))
+            run_step(p, max_norm=1.0, use_stats=True, use_folded=bool(peers))
         assert p.read_clock() == 6
         p.arena.download()
         assert all(p.arena.unchanged(t.param) for t in p.tensors)
@@ -573,6 +576,36 @@ def test_offsets_beyond_32_bits():
     finally:
         buf.close()
         stats.close()
+
+
+def test_more_elements_than_one_launch_takes():
+    """A step over more than 2^33 elements goes out in several launches; the places on both sides of the seam, and the last."""
+    n = (1 << 33) + 4096 + 77
+    grad, param, codes = hip.DeviceBuffer(n * 2), hip.DeviceBuffer(n * 2), hip.DeviceBuffer(n * 2 + 256)
+    scales = hip.DeviceBuffer(2 * (n // BLOCK + 1) * 4)
+    try:
+        for b, byte in ((grad, 0x3C), (param, 0x3D), (codes, 0x30), (scales, 0x3B)):
+            hip.memset(b.ptr, byte, b.nbytes)
+        scale = np.frombuffer(b"\x3b" * 4, np.float32).astype(np.float64)[0]
+        g, p0 = (float(decode(np.array([x], np.uint16), BF16)[0]) for x in (0x3C3C, 0x3D3D))
+        plan = mc.StepPlan(mc.StepLayout(BF16, BF16, NONE, 8, 0, 0), [mc.StepTensor(
+            grad=grad.ptr, param=param.ptr, exp_avg=codes.ptr, exp_avg_sq=codes.ptr + n, exp_avg_scale=scales.ptr,
+            exp_avg_sq_scale=scales.ptr + (n // BLOCK + 1) * 4, size=n, weight_decay=0.5)])
+        ok(mc.xccl_mem_component_adamw(plan.handle, mc.AdamwArgs(lr=0.01, beta1=0.9, beta2=0.95, eps=1e-8, grad_scale=1.0, step=3),
+                                       MemType.ROCM))
+        plan.close()
+        m = 0.9 * E4M3[0x30] * scale + 0.1 * g
+        v = 0.95 * (E4M3[0x30] * scale) ** 2 + 0.05 * g * g
+        p = p0 * (1 - 0.005) - 0.01 / (1 - 0.9 ** 3) * m / (np.sqrt(v / (1 - 0.95 ** 3)) + 1e-8)
+        for at in (0, (1 << 32) - 8, (1 << 33) - 1032, (1 << 33) - 8, (1 << 33) + 1016, n - 16):
+            got = decode(param.download(np.uint16, 16, 2 * at), BF16)
+            assert_near(got, np.full(16, p), HALF[BF16] * abs(p) + 32 * U * (abs(p) + p0), "parameter at %d" % at)
+        for at in (0, 1 << 33, n - 16):
+            s = scales.download(np.float32, 1, at // BLOCK * 4).astype(np.float64)[0]
+            assert_near(E4M3[codes.download(np.uint8, 16, at)] * s, np.full(16, m), 2.0 ** -4 * m * SLACK, "exp_avg at %d" % at)
+    finally:
+        for b in (grad, param, codes, scales):
+            b.close()
 
 
 @pytest.mark.parametrize("bits", [32, 8])

@@ -183,7 +183,7 @@ GOOD = dict(lr=1e-3, beta1=0.9, beta2=0.95, eps=1e-8, grad_scale=1.0, max_norm=0
 
 @pytest.mark.parametrize("change", [
     dict(lr=-1.0), dict(lr=math.nan), dict(lr=math.inf), dict(beta1=1.0), dict(beta1=-0.1), dict(beta1=math.nan), dict(beta2=1.0),
-    dict(beta2=math.nan), dict(eps=0.0), dict(eps=1e-39), dict(eps=math.nan), dict(eps=math.inf), dict(grad_scale=0.0),
+    dict(beta2=math.nan), dict(eps=0.0), dict(eps=1e-39), dict(eps=math.nan), dict(eps=math.inf), dict(grad_scale=0.0), dict(grad_scale=1e-39),
     dict(grad_scale=-1.0), dict(grad_scale=math.nan), dict(grad_scale=math.inf), dict(max_norm=-1.0), dict(max_norm=math.nan),
     dict(max_norm=math.inf), dict(max_norm=1.0), dict(step=0), dict(stats=BASE + 4), dict(clock=BASE + 4), dict(use_folded=1),
 ], ids=str)

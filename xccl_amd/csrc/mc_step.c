@@ -240,11 +240,12 @@ static uint32_t step_shift(const xccl_rocm_step_layout_t *l, const xccl_rocm_ste
 /* Lays the tables out in host memory, and on the device in one allocation. */
 static xccl_status_t step_build(xccl_rocm_step_plan_t *plan, const xccl_rocm_step_tensor_t *tensors, size_t count)
 {
-    size_t        i, entries = 0, chunks = 0, bytes, at_chunks, at_partials, at_arrivals, at_scalars;
+    size_t        i, entries = 0, chunks = 0, bytes, at_chunks, at_pieces, at_partials, at_arrivals, at_scalars;
     uint32_t      k;
     char         *image;
     step_entry_t *e;
     step_chunk_t *c;
+    step_piece_t *g;
     void         *stream = NULL;
     xccl_status_t st;
 
@@ -260,7 +261,8 @@ static xccl_status_t step_build(xccl_rocm_step_plan_t *plan, const xccl_rocm_ste
         return XCCL_ERR_INVALID_PARAM;
     }
     at_chunks   = step_up(entries * sizeof(*e));
-    at_partials = at_chunks + step_up(chunks * sizeof(*c));
+    at_pieces   = at_chunks + step_up(chunks * sizeof(*c));
+    at_partials = at_pieces + (plan->layout.n_peers == 0 ? step_up(chunks * sizeof(*g)) : 0);
     at_arrivals = at_partials + STEP_FOLD_GRID * sizeof(step_partial_t);
     at_scalars  = at_arrivals + step_up(STEP_ARRIVAL_BYTES);
     bytes       = at_scalars + 256;
@@ -270,6 +272,7 @@ static xccl_status_t step_build(xccl_rocm_step_plan_t *plan, const xccl_rocm_ste
     }
     e = (step_entry_t *)image;
     c = (step_chunk_t *)(image + at_chunks);
+    g = (step_piece_t *)(image + at_pieces);
     for (i = 0, entries = 0; i < count; i++) {
         const xccl_rocm_step_tensor_t *t = &tensors[i];
 
@@ -283,7 +286,14 @@ static xccl_status_t step_build(xccl_rocm_step_plan_t *plan, const xccl_rocm_ste
             .size = t->size, .decay = t->weight_decay, .shift = step_shift(&plan->layout, t),
         };
         for (k = 0; k < (t->size + e[entries].shift + STEP_CHUNK - 1) / STEP_CHUNK; k++) {
+            const size_t end  = (size_t)(k + 1) * STEP_CHUNK - e[entries].shift;
+            const size_t from = k == 0 ? 0 : end - STEP_CHUNK;
+
             *c++ = (step_chunk_t){.entry = (uint32_t)entries, .index = k};
+            if (plan->layout.n_peers == 0) {
+                *g++ = (step_piece_t){.grad = e[entries].grad + from * step_dt_size(plan->layout.grad_dtype),
+                                      .left = (end < t->size ? end : t->size) - from};
+            }
         }
         entries++;
     }
@@ -304,9 +314,10 @@ static xccl_status_t step_build(xccl_rocm_step_plan_t *plan, const xccl_rocm_ste
     plan->chunks      = chunks;
     plan->entries     = (step_entry_t *)plan->memory;
     plan->chunk_table = (step_chunk_t *)(plan->memory + at_chunks);
+    plan->pieces      = (step_piece_t *)(plan->memory + at_pieces);
     plan->partials    = (step_partial_t *)(plan->memory + at_partials);
     plan->arrivals    = (uint32_t *)(plan->memory + at_arrivals);
-    plan->zero        = (double *)(plan->memory + at_scalars + 128);
+    plan->zeros       = (double *)(plan->memory + at_scalars + 128);
     plan->scalars     = (step_scalars_t *)(plan->memory + at_scalars);
     return st;
 }
@@ -454,7 +465,7 @@ static xccl_status_t step_adamw(xccl_rocm_step_plan_t *plan, const xccl_rocm_ada
     }
     /* eps is added in 32 bits and keeps the quotient finite where m and v are 0: it has to be a normal number there */
     if (step_outside(a->beta1, 0, 1) || step_outside(a->beta2, 0, 1) || step_outside(a->eps, FLT_MIN, FLT_MAX) ||
-        step_outside(a->grad_scale, DBL_MIN, FLT_MAX) || step_outside(a->max_norm, 0, INFINITY) ||
+        step_outside(a->grad_scale, FLT_MIN, FLT_MAX) || step_outside(a->max_norm, 0, INFINITY) ||
         (a->clock == NULL && (step_outside(a->lr, 0, FLT_MAX) || a->step == 0)) ||
         (a->max_norm > 0 && a->stats == NULL) || (uintptr_t)a->stats % sizeof(double) != 0 ||
         (uintptr_t)a->clock % sizeof(double) != 0 || (a->use_folded && !plan->writes_fold)) {

@@ -221,6 +221,7 @@ constexpr uint32_t kNormWaves = 4; // of a workgroup
 struct NormArgs {
     const step_entry_t *entries;
     const step_chunk_t *chunks;
+    const step_piece_t *pieces;
     step_partial_t     *partials;
     uint32_t           *arrivals;
     double             *stats;
@@ -302,18 +303,12 @@ __device__ __forceinline__ void norm_finish(const NormArgs &a, NormTotal t)
 // Squares are summed in 64 bits: in 32 they would overflow from 1.8e19 and
 // vanish below 1e-23.  Two chains of additions, one for each half of the lane's elements.
 struct NormSum {
-    double   even = 0, odd = 0;
-    uint32_t bad = 0;
+    double even = 0, odd = 0;
     __device__ __forceinline__ void add(float x, bool is_odd)
     {
         const double d = (double)x;
         double      &s = is_odd ? odd : even;
         s              = __builtin_fma(d, d, s);
-        bad += !__builtin_isfinite(x);
-    }
-    __device__ __forceinline__ NormTotal total() const
-    {
-        return {even + odd, bad};
     }
 };
 
@@ -337,6 +332,24 @@ template <typename G> struct NormChunk {
         }
     }
 
+    __device__ __forceinline__ uint32_t bad() const
+    {
+        typedef G V __attribute__((ext_vector_type(16 / sizeof(G))));
+        uint32_t  n = 0;
+#pragma unroll
+        for (int i = 0; i < Loads; ++i) {
+            const V v = __builtin_bit_cast(V, x[i]);
+#pragma unroll
+            for (uint32_t k = 0; k < 16 / sizeof(G); ++k) {
+                n += !__builtin_isfinite((float)v[k]);
+            }
+        }
+        if constexpr (sizeof(G) == 2) {
+            n += !__builtin_isfinite((float)__builtin_bit_cast(G, last));
+        }
+        return n;
+    }
+
     __device__ __forceinline__ void sum(NormSum &s) const
     {
         typedef G V __attribute__((ext_vector_type(16 / sizeof(G))));
@@ -354,33 +367,27 @@ template <typename G> struct NormChunk {
     }
 };
 
-struct Piece {
-    const char *base;
-    uint32_t    left; // elements; 0 behind the last chunk
-};
-
-__device__ __forceinline__ step_chunk_t norm_chunk(const NormArgs &a, uint32_t c)
+// The piece of chunk c, or of the last chunk; a wave whose chunk lies behind that
+// masks its elements when it uses them, not here, where that would wait for them.
+__device__ __forceinline__ step_piece_t norm_piece(const NormArgs &a, uint32_t c)
 {
-    return a.chunks[c < a.n_chunks ? c : a.n_chunks - 1];
+    const auto   at = (const __attribute__((address_space(4))) step_piece_t *)a.pieces + (c < a.n_chunks ? c : a.n_chunks - 1);
+    step_piece_t p;
+    p.grad = at->grad;
+    p.left = at->left;
+    return p;
 }
 
-__device__ __forceinline__ Piece norm_piece(const NormArgs &a, uint32_t c, step_chunk_t chunk, uint32_t elem)
+__device__ __forceinline__ uint32_t norm_left(const NormArgs &a, const step_piece_t &p, uint32_t c)
 {
-    const step_entry_t *t    = a.entries + chunk.entry;
-    const int64_t       from = (int64_t)chunk.index * STEP_CHUNK - t->shift;
-    const int64_t       to   = from + STEP_CHUNK < (int64_t)t->size ? from + STEP_CHUNK : (int64_t)t->size;
-    const int64_t       at   = from < 0 ? 0 : from;
-    Piece               p;
-    p.base = t->grad + at * elem;
-    p.left = c < a.n_chunks ? (uint32_t)(to - at) : 0u;
-    return p;
+    return (uint32_t)p.left & (uint32_t)(((uint64_t)c - a.n_chunks) >> 32); // all ones up to the last chunk: no branch
 }
 
 // One vector per tensor.  Which chunks a wave takes and the order of every sum
 // depend on the plan alone, so equal gradients give equal results.  A wave
-// requests 4 KiB before it sums up the last 4 KiB, has read the tensor's entry
-// for that a round before, and the table's a round before that: no address is
-// waited for.
+// requests 4 KiB before it sums up the last 4 KiB, and has read where they lie
+// a round before that.  The scheduling barriers keep it so: left alone, the
+// compiler puts the requests behind the sums.
 template <typename G>
 __global__ void __launch_bounds__(kNormWaves * 64) grad_norm_kernel(const NormArgs a)
 {
@@ -390,41 +397,53 @@ __global__ void __launch_bounds__(kNormWaves * 64) grad_norm_kernel(const NormAr
     NormSum            s;
     if (a.n_chunks != 0) {
         NormChunk<G> x[K], y[K];
-        Piece        piece[K];
-        step_chunk_t chunk[K];
-        uint32_t     c = wave * K; // what x holds; piece is `step` further, chunk `2 * step`
-#pragma unroll
-        for (uint32_t k = 0; k < K; ++k) {
-            piece[k] = norm_piece(a, c + k, norm_chunk(a, c + k), sizeof(G));
-            chunk[k] = norm_chunk(a, c + step + k);
-        }
-        auto advance = [&](NormChunk<G>(&to)[K], uint32_t at) {
+        step_piece_t piece[K];
+        uint32_t     c = wave * K; // what x holds; piece is `step` further
+        auto request = [&](NormChunk<G>(&to)[K], uint32_t at) {
 #pragma unroll
             for (uint32_t k = 0; k < K; ++k) {
-                to[k].load(piece[k].base, piece[k].left);
+                to[k].load(piece[k].grad, norm_left(a, piece[k], at + k));
             }
 #pragma unroll
             for (uint32_t k = 0; k < K; ++k) {
-                piece[k] = norm_piece(a, at + step + k, chunk[k], sizeof(G));
-                chunk[k] = norm_chunk(a, at + 2 * step + k);
+                piece[k] = norm_piece(a, at + step + k);
             }
+            __builtin_amdgcn_sched_barrier(0);
         };
         auto sum = [&](const NormChunk<G>(&of)[K]) {
 #pragma unroll
             for (uint32_t k = 0; k < K; ++k) {
                 of[k].sum(s);
             }
+            __builtin_amdgcn_sched_barrier(0);
         };
-        advance(x, c);
+#pragma unroll
+        for (uint32_t k = 0; k < K; ++k) {
+            piece[k] = norm_piece(a, c + k);
+        }
+        request(x, c);
         while (c < a.n_chunks) {
-            advance(y, c + step);
+            request(y, c + step);
             sum(x);
-            advance(x, c + 2 * step);
+            request(x, c + 2 * step);
             sum(y);
             c += 2 * step;
         }
     }
-    norm_finish(a, s.total());
+    // 64 bits hold the sum of any number of 32-bit squares: it is finite unless an element is not.  Only then
+    // are those counted, in a second pass of the wave over its chunks, which spares the first a third of its work.
+    NormTotal t = {s.even + s.odd, 0};
+    if (__any(!__builtin_isfinite(t.sum))) {
+        for (uint32_t c = wave * K; c < a.n_chunks; c += step) {
+            for (uint32_t k = 0; k < K; ++k) {
+                const step_piece_t piece = norm_piece(a, c + k);
+                NormChunk<G>       x;
+                x.load(piece.grad, norm_left(a, piece, c + k));
+                t.bad += x.bad();
+            }
+        }
+    }
+    norm_finish(a, t);
 }
 
 // With peers' vectors: a wave folds N tiles at a time, and writes the fold if
@@ -433,7 +452,8 @@ constexpr int      kFoldTiles   = 2;
 constexpr uint32_t kFoldPerChunk = STEP_CHUNK / 256 / kFoldTiles;
 
 template <typename G, bool Full, int N>
-__device__ __forceinline__ void fold_tiles(const NormArgs &a, const step_entry_t &t, const Span *span, NormSum &s)
+__device__ __forceinline__ void fold_tiles(const NormArgs &a, const step_entry_t &t, const Span *span, NormSum &s,
+                                           uint32_t &bad)
 {
     const uint32_t           lane = threadIdx.x & 63;
     Fold<G, Full, true, N>   fold;
@@ -447,6 +467,7 @@ __device__ __forceinline__ void fold_tiles(const NormArgs &a, const step_entry_t
         for (int k = 0; k < 4; ++k) {
             x[k] = (float)(G)x[k];
             s.add(x[k], k & 1);
+            bad += !__builtin_isfinite(x[k]);
         }
         if (a.writes_fold) {
             store4<G, Full, kStepAuxStore<G>>(t.folded, span[i], lane, x);
@@ -463,6 +484,7 @@ __global__ void __launch_bounds__(kNormWaves * 64) fold_norm_kernel(const NormAr
     constexpr int  N    = kFoldTiles;
     const uint32_t wave = blockIdx.x * kNormWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     NormSum        s;
+    uint32_t       bad = 0;
     for (uint32_t u = wave; u < a.n_chunks * kFoldPerChunk; u += a.grid * kNormWaves) {
         const step_chunk_t chunk = a.chunks[u / kFoldPerChunk];
         const step_entry_t t     = a.entries[chunk.entry];
@@ -475,15 +497,15 @@ __global__ void __launch_bounds__(kNormWaves * 64) fold_norm_kernel(const NormAr
             have += span[i].left;
         }
         if (have == 256 * N) {
-            fold_tiles<G, true, N>(a, t, span, s);
+            fold_tiles<G, true, N>(a, t, span, s, bad);
         } else {
             for (int i = 0; i < N; ++i) {
                 const Span one = tile_span(t, first + i);
-                fold_tiles<G, false, 1>(a, t, &one, s);
+                fold_tiles<G, false, 1>(a, t, &one, s, bad);
             }
         }
     }
-    norm_finish(a, s.total());
+    norm_finish(a, {s.even + s.odd, bad});
 }
 
 // ---- AdamW ------------------------------------------------------------------
@@ -501,7 +523,7 @@ struct AdamwKernelArgs {
     const step_scalars_t *from;  // device: read instead of `s` if not NULL
     const double         *stats; // device, or NULL
     step_scalars_t        s;
-    double                zero;  // read instead of stats[1] if there is no stats
+    double                zero[2]; // read instead of *stats if there is none
     double                grad_scale, max_norm;
     float                 g;     // factor of the folded gradient, where it is not clipped
     uint32_t              clip;
@@ -533,12 +555,19 @@ __host__ __device__ inline void step_rate(step_scalars_t &s, double beta1, doubl
     s.inv_c2 = (float)(1 / sqrt(1 - power(beta2, t)));
 }
 
+// Whether the whole step is skipped, by the bits of its stats: an element was
+// not finite, or the sum of squares is no such sum (negative, infinite, NaN).
+__device__ __forceinline__ bool step_skips(uint64_t sum, uint64_t bad)
+{
+    return (bad << 1) != 0 || (sum >> 52) >= 0x7ff;
+}
+
 // Ahead of a step that has a clock: reads it for the step, and counts the step
-// unless it is going to be skipped.  All loads go out at once, stats[1] from a
-// place that holds 0 if there is none.
+// unless it is going to be skipped.  All loads go out at once, the stats from a
+// place that holds zeros if there are none.
 struct ClockArgs {
     xccl_rocm_step_clock_t *clock;
-    const double           *bad;
+    const double           *stats;
     step_scalars_t         *to;
     double                  beta1, beta2;
 };
@@ -547,11 +576,11 @@ __global__ void step_clock_kernel(const ClockArgs a)
 {
     const double   lr  = a.clock->lr;
     const uint64_t t   = a.clock->steps + 1;
-    const double   bad = *a.bad;
+    const uint64_t sum = __builtin_bit_cast(uint64_t, a.stats[0]), bad = __builtin_bit_cast(uint64_t, a.stats[1]);
     step_scalars_t s;
     step_rate(s, a.beta1, a.beta2, lr, t);
     *a.to = s;
-    if (bad == 0) {
+    if (!step_skips(sum, bad)) {
         a.clock->steps = t;
     }
 }
@@ -698,8 +727,9 @@ __global__ void __launch_bounds__(64) adamw_kernel(const AdamwKernelArgs a)
     const Constant args = (Constant)__builtin_amdgcn_kernarg_segment_ptr();
     const auto     from = (const __attribute__((address_space(4))) step_scalars_t *)(
         a.from != nullptr ? (Constant)a.from : args + offsetof(AdamwKernelArgs, s));
-    const uint64_t bad  = *(const __attribute__((address_space(4))) uint64_t *)(
-        a.stats != nullptr ? (Constant)(a.stats + 1) : args + offsetof(AdamwKernelArgs, zero));
+    const auto     stats = (const __attribute__((address_space(4))) uint64_t *)(
+        a.stats != nullptr ? (Constant)a.stats : args + offsetof(AdamwKernelArgs, zero));
+    const bool     skip = step_skips(stats[0], stats[1]);
     step_scalars_t s;
     s.lr     = from->lr;
     s.size   = from->size;
@@ -707,8 +737,8 @@ __global__ void __launch_bounds__(64) adamw_kernel(const AdamwKernelArgs a)
     const step_chunk_t chunk = a.chunks[blockIdx.x / kStepTiles];
     const step_entry_t t     = a.entries[chunk.entry];
     Span               span  = tile_span(t, (uint64_t)chunk.index * kStepTiles + blockIdx.x % kStepTiles);
-    if (bad << 1 != 0) {
-        span.left = 0; // not 0 of either sign: a gradient is not finite, nothing is read or written
+    if (skip) {
+        span.left = 0; // nothing is read or written
     }
     if (span.left == kStepTile) {
         adamw_tile<P, G, Eight, Peers, true>(a, s, t, span);

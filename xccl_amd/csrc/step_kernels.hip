@@ -9,15 +9,20 @@ using namespace xccl_rocm;
 
 namespace {
 
-xccl_status_t launched(const char *what)
+xccl_status_t launch(const char *what, const void *fn, unsigned grid, unsigned block, void *args, unsigned lds, void *hip_stream)
 {
-    const hipError_t e = hipGetLastError();
+    void            *argv[1] = {args};
+    const hipError_t e       = hipLaunchKernel(fn, dim3(grid), dim3(block), argv, lds, (hipStream_t)hip_stream);
     if (e != hipSuccess) {
         fprintf(stderr, "xccl mc_rocm: launch of %s failed: %s\n", what, hipGetErrorString(e));
         return XCCL_ERR_NO_MESSAGE;
     }
     return XCCL_OK;
 }
+
+// Chunks of one launch of the step, 2^33 elements: a grid may not have 2^32 threads.
+constexpr size_t kStepLaunchChunks = (size_t)1 << 23;
+static_assert(kStepLaunchChunks * kStepTiles * 64 < (size_t)1 << 32, "threads of a launch");
 
 typedef void (*AdamwKernel)(AdamwKernelArgs);
 
@@ -85,6 +90,7 @@ xccl_status_t step_launch_grad_norm(const xccl_rocm_step_plan_t *plan, double *s
     NormArgs   a;
     a.entries     = plan->entries;
     a.chunks      = plan->chunk_table;
+    a.pieces      = plan->pieces;
     a.partials    = plan->partials;
     a.arrivals    = plan->arrivals;
     a.stats       = stats;
@@ -97,32 +103,24 @@ xccl_status_t step_launch_grad_norm(const xccl_rocm_step_plan_t *plan, double *s
     const uint32_t want  = (units + kNormWaves - 1) / kNormWaves;
     const uint32_t most  = fold ? STEP_FOLD_GRID : STEP_NORM_GRID;
     a.grid               = want < 1 ? 1 : want < most ? want : most;
-    const dim3        grid(a.grid), block(kNormWaves * 64);
-    const hipStream_t s = (hipStream_t)hip_stream;
+    const void *fn;
     switch ((int)plan->layout.grad_dtype) {
-    case XCCL_DT_FLOAT32:
-        hipLaunchKernelGGL(fold ? fold_norm_kernel<float> : grad_norm_kernel<float>, grid, block, 0, s, a);
-        break;
-    case XCCL_DT_FLOAT16:
-        hipLaunchKernelGGL(fold ? fold_norm_kernel<_Float16> : grad_norm_kernel<_Float16>, grid, block, 0, s, a);
-        break;
-    default:
-        hipLaunchKernelGGL(fold ? fold_norm_kernel<__bf16> : grad_norm_kernel<__bf16>, grid, block, 0, s, a);
-        break;
+    case XCCL_DT_FLOAT32: fn = fold ? (const void *)fold_norm_kernel<float> : (const void *)grad_norm_kernel<float>; break;
+    case XCCL_DT_FLOAT16: fn = fold ? (const void *)fold_norm_kernel<_Float16> : (const void *)grad_norm_kernel<_Float16>; break;
+    default:              fn = fold ? (const void *)fold_norm_kernel<__bf16> : (const void *)grad_norm_kernel<__bf16>; break;
     }
-    return launched("grad_norm");
+    return launch("grad_norm", fn, a.grid, kNormWaves * 64, &a, 0, hip_stream);
 }
 
 xccl_status_t step_launch_adamw(const xccl_rocm_step_plan_t *plan, const xccl_rocm_adamw_args_t *args, void *hip_stream)
 {
     const xccl_rocm_step_layout_t &l = plan->layout;
-    const hipStream_t              s = (hipStream_t)hip_stream;
     AdamwKernelArgs                a;
     a.entries     = plan->entries;
-    a.chunks      = plan->chunk_table;
     a.from        = nullptr;
     a.stats       = args->stats;
-    a.zero        = 0;
+    a.zero[0]     = 0;
+    a.zero[1]     = 0;
     a.grad_scale  = args->grad_scale;
     a.max_norm    = args->max_norm;
     a.g           = (float)args->grad_scale;
@@ -139,12 +137,11 @@ xccl_status_t step_launch_adamw(const xccl_rocm_step_plan_t *plan, const xccl_ro
     if (args->clock != nullptr) {
         ClockArgs c;
         c.clock = args->clock;
-        c.bad   = args->stats != nullptr ? args->stats + 1 : plan->zero;
+        c.stats = args->stats != nullptr ? args->stats : plan->zeros;
         c.to    = plan->scalars;
         c.beta1 = args->beta1;
         c.beta2 = args->beta2;
-        hipLaunchKernelGGL(step_clock_kernel, dim3(1), dim3(1), 0, s, c);
-        const xccl_status_t st = launched("the step's clock");
+        const xccl_status_t st = launch("the step's clock", (const void *)step_clock_kernel, 1, 1, &c, 0, hip_stream);
         if (st != XCCL_OK) {
             return st;
         }
@@ -153,12 +150,16 @@ xccl_status_t step_launch_adamw(const xccl_rocm_step_plan_t *plan, const xccl_ro
     } else {
         step_rate(a.s, args->beta1, args->beta2, args->lr, args->step);
     }
-    if (plan->chunks == 0) {
-        return XCCL_OK;
+    const AdamwKernel k   = adamw_by_types(l.param_dtype, l.grad_dtype, l.state_bits == 8, a.n_peers != 0);
+    const unsigned    lds = adamw_lds(plan, a.n_peers);
+    xccl_status_t     st  = XCCL_OK;
+    for (size_t done = 0; done < plan->chunks && st == XCCL_OK; done += kStepLaunchChunks) {
+        const size_t left = plan->chunks - done;
+        a.chunks          = plan->chunk_table + done;
+        st = launch("adamw", (const void *)k, (unsigned)(left < kStepLaunchChunks ? left : kStepLaunchChunks) * kStepTiles, 64,
+                    &a, lds, hip_stream);
     }
-    const AdamwKernel k = adamw_by_types(l.param_dtype, l.grad_dtype, l.state_bits == 8, a.n_peers != 0);
-    hipLaunchKernelGGL(k, dim3((unsigned)plan->chunks * kStepTiles), dim3(64), adamw_lds(plan, a.n_peers), s, a);
-    return launched("adamw");
+    return st;
 }
 
 } // extern "C"

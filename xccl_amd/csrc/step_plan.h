@@ -36,7 +36,13 @@ typedef struct step_chunk {
     uint32_t entry;
     uint32_t index;
 } step_chunk_t;
-#define STEP_MAX_CHUNKS 0x1fffffffu /* a step launches four workgroups for each */
+/* Where the local gradient vector's part of a chunk lies, and its elements: for grad_norm without peers, which does so
+ * little with each chunk that looking up chunk, entry and address one after the other would take longer than that. */
+typedef struct step_piece {
+    const char *grad;
+    uint64_t    left;
+} step_piece_t;
+#define STEP_MAX_CHUNKS 0x1fffffffu /* so that the kernels' counts of chunks and their parts stay within 32 bits */
 
 /* grad_norm runs at most this many workgroups, without and with peers; each leaves one partial result. */
 #define STEP_NORM_GRID 512u
@@ -66,9 +72,10 @@ struct xccl_rocm_step_plan {
     char                   *memory;   /* device: the one allocation behind the pointers below */
     step_entry_t           *entries;
     step_chunk_t           *chunk_table;
+    step_piece_t           *pieces;   /* one per chunk; without peers only */
     step_partial_t         *partials; /* STEP_FOLD_GRID of them */
     uint32_t               *arrivals; /* workgroups of grad_norm that are through (STEP_ARRIVAL_BYTES); zero between launches */
-    double                 *zero;     /* holds 0 */
+    double                 *zeros;    /* two of them: stats of a step that has none */
     step_scalars_t         *scalars;  /* of the step that runs, where there is a clock */
 };
 

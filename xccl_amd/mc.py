@@ -258,11 +258,11 @@ def benchkit_lib():
     return _datagen_lib
 
 
+_STATUS = {int(s): s for s in Status}
+
+
 def _st(code) -> Status:
-    try:
-        return Status(code)
-    except ValueError:
-        return code
+    return _STATUS.get(code, code)
 
 
 class Stream:
@@ -389,11 +389,14 @@ def xccl_mem_component_grad_norm(plan, stats, mem_type) -> Status:
     return _st(dispatch_lib().xccl_mem_component_grad_norm(plan, stats, int(mem_type)))
 
 
+def _step_nb(fn, plan, arg, mem_type, stream, want_event):
+    ev = _vp() if want_event else None
+    st = fn(plan, arg, mem_type, stream.ref() if stream else None, _c.byref(ev) if want_event else None)
+    return _st(st), ev.value if want_event else None
+
+
 def xccl_mem_component_grad_norm_nb(plan, stats, mem_type, stream=None, want_event=True):
-    ev = _vp()
-    st = dispatch_lib().xccl_mem_component_grad_norm_nb(plan, stats, int(mem_type), stream.ref() if stream else None,
-                                                        _c.byref(ev) if want_event else None)
-    return _st(st), ev.value
+    return _step_nb(dispatch_lib().xccl_mem_component_grad_norm_nb, plan, stats, mem_type, stream, want_event)
 
 
 def xccl_mem_component_adamw(plan, args: AdamwArgs, mem_type) -> Status:
@@ -401,11 +404,7 @@ def xccl_mem_component_adamw(plan, args: AdamwArgs, mem_type) -> Status:
 
 
 def xccl_mem_component_adamw_nb(plan, args: AdamwArgs, mem_type, stream=None, want_event=True):
-    ev = _vp()
-    st = dispatch_lib().xccl_mem_component_adamw_nb(plan, _c.byref(args), int(mem_type),
-                                                    stream.ref() if stream else None,
-                                                    _c.byref(ev) if want_event else None)
-    return _st(st), ev.value
+    return _step_nb(dispatch_lib().xccl_mem_component_adamw_nb, plan, _c.byref(args), mem_type, stream, want_event)
 
 
 class StepPlan:
