@@ -206,7 +206,7 @@ def test_calls_refused():
     assert mc.xccl_mem_component_step_plan_destroy(None, MemType.ROCM) == INVALID
 
 
-@pytest.mark.parametrize("mt", [MemType.HOST, MemType.CUDA, MemType.LAST, 99, -1], ids=str)
+@pytest.mark.parametrize("mt", [MemType.HOST, MemType.LAST, 99, -1], ids=str)
 def test_no_component(mt):
     args = mc.AdamwArgs(**GOOD)
     assert mc.xccl_mem_component_step_plan_create(layout(), [], mt) == (UNSUPPORTED, None)

@@ -525,8 +525,7 @@ struct AdamwKernelArgs {
     step_scalars_t        s;
     double                zero[2]; // read instead of *stats if there is none
     double                grad_scale, max_norm;
-    float                 g;     // factor of the folded gradient, where it is not clipped
-    uint32_t              clip;
+    uint32_t              clip; // work the factor out here: there is a norm, and no clock
     size_t                peer_stride;
     uint32_t              n_peers;
     uint32_t              use_folded;
@@ -569,8 +568,15 @@ struct ClockArgs {
     xccl_rocm_step_clock_t *clock;
     const double           *stats;
     step_scalars_t         *to;
-    double                  beta1, beta2;
+    double                  beta1, beta2, grad_scale, max_norm;
 };
+
+// The factor of the folded gradient.
+__device__ __forceinline__ float step_factor(double sum, double grad_scale, double max_norm)
+{
+    const double k = max_norm / (sqrt(sum) * grad_scale + 1e-6);
+    return (float)(max_norm > 0 && k < 1 ? grad_scale * k : grad_scale);
+}
 
 __global__ void step_clock_kernel(const ClockArgs a)
 {
@@ -579,6 +585,7 @@ __global__ void step_clock_kernel(const ClockArgs a)
     const uint64_t sum = __builtin_bit_cast(uint64_t, a.stats[0]), bad = __builtin_bit_cast(uint64_t, a.stats[1]);
     step_scalars_t s;
     step_rate(s, a.beta1, a.beta2, lr, t);
+    s.g   = step_factor(__builtin_bit_cast(double, sum), a.grad_scale, a.max_norm);
     *a.to = s;
     if (!step_skips(sum, bad)) {
         a.clock->steps = t;
@@ -617,12 +624,10 @@ __device__ __forceinline__ float nearest_sqrt(float x)
     return __builtin_fmaf(-above, s, x) > 0 ? above : r;
 }
 
-// Four e4m3 codes of x, and the power of two they are to be multiplied with.
+// The power of two that a block's values are divided by for their e4m3 codes.
 // Magnitudes order as their bits do; adding 0x1fffff carries into the exponent
 // iff the mantissa is above 1.75, i.e. iff 448 of 2^(exponent - 8) is too small.
-// Positive: where `of`, the square of x, is above zero the code is too.
-template <bool Positive>
-__device__ __forceinline__ uint32_t quantize(f32x4 x, f32x4 of, float &scale)
+__device__ __forceinline__ float block_scale(f32x4 x)
 {
     uint32_t most = 0;
 #pragma unroll
@@ -631,28 +636,39 @@ __device__ __forceinline__ uint32_t quantize(f32x4 x, f32x4 of, float &scale)
         const uint32_t b  = __builtin_bit_cast(uint32_t, xk) & 0x7fffffffu;
         most = b > most ? b : most;
     }
-    most = wave_max(most);
-    const int   up  = (int)((most + 0x1fffffu) >> 23) - 8;
-    const int   e   = up < 1 ? 1 : up;
-    const float inv = __builtin_bit_cast(float, (254 - e) << 23);
-    scale = __builtin_bit_cast(float, e << 23);
-    f32x4 y;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        y[k] = x[k] * inv;
-        if (Positive) {
-            y[k] = of[k] > 0 && y[k] < 0x1p-9f ? 0x1p-9f : y[k];
-        }
-    }
-    int code = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], code, true);
+    const int e = (int)((wave_max(most) + 0x1fffffu) >> 23) - 8;
+    return __builtin_bit_cast(float, (e < 1 ? 1 : e) << 23);
 }
 
+// Codes of four values.  The instruction divides by the scale's power of two.
+__device__ __forceinline__ uint32_t quantize(f32x4 x, float scale)
+{
+    typedef short s16x2 __attribute__((ext_vector_type(2)));
+    s16x2 c = {0, 0};
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, x[0], x[1], scale, false);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, x[2], x[3], scale, true);
+    return __builtin_bit_cast(uint32_t, c);
+}
+
+// And back, by a product, so that a scale which some other code wrote need not be a power of two.
 __device__ __forceinline__ f32x4 dequantize(uint32_t codes, float scale)
 {
     const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false);
     const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true);
     return f32x4{lo[0] * scale, lo[1] * scale, hi[0] * scale, hi[1] * scale};
+}
+
+// r = sqrt(v), but nothing above zero below the smallest code.  As integers, which leaves a NaN what it is.
+__device__ __forceinline__ f32x4 above_zero(f32x4 r, f32x4 v, float scale)
+{
+    const uint32_t least = __builtin_bit_cast(uint32_t, scale * 0x1p-9f);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float    rk = r[k];
+        const uint32_t b  = __builtin_bit_cast(uint32_t, rk), l = v[k] > 0 ? least : 0u;
+        r[k] = __builtin_bit_cast(float, b > l ? b : l);
+    }
+    return r;
 }
 
 template <typename P, typename G, bool Eight, bool Peers, bool Full>
@@ -677,10 +693,9 @@ __device__ __forceinline__ void adamw_tile(const AdamwKernelArgs &a, const step_
         v = load4<float, Full>(t.sq, span, lane);
     }
     const float keep   = (float)(1 - s.lr * t.decay);
-    float       factor = a.g;
+    float       factor = s.g;
     if (a.clip) {
-        const double k = a.max_norm / (sqrt(*(const __attribute__((address_space(4))) double *)a.stats) * a.grad_scale + 1e-6);
-        factor         = (float)(a.grad_scale * (k < 1 ? k : 1));
+        factor = step_factor(*(const __attribute__((address_space(4))) double *)a.stats, a.grad_scale, a.max_norm);
     }
     fold.end();
     const f32x4 g = fold.sum[0] * factor;
@@ -698,7 +713,8 @@ __device__ __forceinline__ void adamw_tile(const AdamwKernelArgs &a, const step_
         // that the parameter sees.  The square root that is stored as a code is the correctly rounded one: a block's
         // scale hangs on it.
         r[k] = Eight ? nearest_sqrt(vk) : __builtin_amdgcn_sqrtf(vk);
-        p[k] = p[k] * keep - s.size * (m[k] * __builtin_amdgcn_rcpf(r[k] * s.inv_c2 + a.eps));
+        const float u = m[k] * __builtin_amdgcn_rcpf(__builtin_fmaf(r[k], s.inv_c2, a.eps));
+        p[k]          = __builtin_fmaf(-s.size, u, p[k] * keep);
     }
     store4<P, Full, kStepAuxStore<G>>(t.param, span, lane, p);
     if (a.copy == 1) {
@@ -707,8 +723,10 @@ __device__ __forceinline__ void adamw_tile(const AdamwKernelArgs &a, const step_
         store4<__bf16, Full, kStepAuxStore<G>>(t.copy, span, lane, p);
     }
     if constexpr (Eight) {
-        store_codes<Full, kStepAuxStore<G>>(t.avg, span, lane, quantize<false>(m, m, m_scale));
-        store_codes<Full, kStepAuxStore<G>>(t.sq, span, lane, quantize<true>(r, v, r_scale));
+        m_scale = block_scale(m);
+        r_scale = block_scale(r);
+        store_codes<Full, kStepAuxStore<G>>(t.avg, span, lane, quantize(m, m_scale));
+        store_codes<Full, kStepAuxStore<G>>(t.sq, span, lane, quantize(above_zero(r, v, r_scale), r_scale));
         if (lane == 0) {
             ((STEP_GLOBAL float *)t.avg_scale)[block] = m_scale;
             ((STEP_GLOBAL float *)t.sq_scale)[block]  = r_scale;
@@ -734,6 +752,7 @@ __global__ void __launch_bounds__(64) adamw_kernel(const AdamwKernelArgs a)
     s.lr     = from->lr;
     s.size   = from->size;
     s.inv_c2 = from->inv_c2;
+    s.g      = from->g;
     const step_chunk_t chunk = a.chunks[blockIdx.x / kStepTiles];
     const step_entry_t t     = a.entries[chunk.entry];
     Span               span  = tile_span(t, (uint64_t)chunk.index * kStepTiles + blockIdx.x % kStepTiles);

@@ -123,8 +123,8 @@ xccl_status_t step_launch_adamw(const xccl_rocm_step_plan_t *plan, const xccl_ro
     a.zero[1]     = 0;
     a.grad_scale  = args->grad_scale;
     a.max_norm    = args->max_norm;
-    a.g           = (float)args->grad_scale;
-    a.clip        = args->max_norm > 0;
+    a.clip        = args->max_norm > 0 && args->clock == nullptr;
+    a.s.g         = (float)args->grad_scale;
     a.peer_stride = l.peer_stride;
     a.n_peers     = args->use_folded ? 0 : l.n_peers;
     a.use_folded  = args->use_folded != 0;
@@ -141,6 +141,8 @@ xccl_status_t step_launch_adamw(const xccl_rocm_step_plan_t *plan, const xccl_ro
         c.to    = plan->scalars;
         c.beta1 = args->beta1;
         c.beta2 = args->beta2;
+        c.grad_scale = args->grad_scale;
+        c.max_norm   = args->max_norm;
         const xccl_status_t st = launch("the step's clock", (const void *)step_clock_kernel, 1, 1, &c, 0, hip_stream);
         if (st != XCCL_OK) {
             return st;

@@ -57,11 +57,12 @@ typedef struct step_partial {
 #define STEP_ARRIVAL_STRIDE 32u
 #define STEP_ARRIVAL_BYTES ((1 + STEP_ARRIVAL_SHARDS) * STEP_ARRIVAL_STRIDE * 4)
 
-/* What depends on step number and rate. */
+/* What depends on step number, rate and norm. */
 typedef struct step_scalars {
     double lr;
     float  size;   /* lr / (1 - beta1^t) */
     float  inv_c2; /* 1 / sqrt(1 - beta2^t) */
+    float  g;      /* factor of the folded gradient */
 } step_scalars_t;
 
 struct xccl_rocm_step_plan {
