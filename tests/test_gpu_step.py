@@ -1,5 +1,8 @@
 """The optimizer step on the GPU against its plain form in 64 bits (step_util.py, where the tolerances come from)."""
 import ctypes
+import os
+import subprocess
+import sys
 import threading
 
 import numpy as np
@@ -11,6 +14,7 @@ from xccl_amd import hip, mc
 from xccl_amd.types import Dt, MemType, Op, Status
 
 pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 # around the lane (4), the tile and block (256), the chunk (4096), and what is left over
 EDGES = [0, 1, 2, 3, 4, 5, 63, 64, 255, 256, 257, 0, 511, 1023, 4095, 4096, 4097, 8193, 12345]
@@ -199,6 +203,31 @@ def test_norm_of_more_chunks_than_workgroups(n):
             check_norm(p)
         finally:
             p.close()
+
+
+@pytest.mark.parametrize("grad", TYPES, ids=NAMES.get)
+@pytest.mark.parametrize("peers", [0, 1])
+def test_norm_counts_everywhere(grad, peers):
+    """Elements that are not finite in the first and last place of tensors, in every part of a wave's rounds: exact count, and
+    the next call on mended gradients is as if nothing had been."""
+    sizes = [3, 4097, 9000001, 1025]
+    plant = [(0, 2, np.nan), (1, 0, np.inf), (1, 4096, -np.inf), (3, 1024, np.nan)]
+    plant += [(2, at, (np.inf, -np.inf, np.nan)[at % 3]) for at in (0, 1, 1023, 1024, 4194303, 4194304, 8388608, 9000000)]
+    p = Problem(sizes, grad, bits=0, peers=peers, fold="own" if peers else None, plant=plant, shift=True)
+    try:
+        grad_norm(p)
+        total, bad = p.read_stats()
+        assert bad == len(plant) and not np.isfinite(total)
+        for k, at, _ in plant:
+            t = p.tensors[k]
+            t.g[-1][at] = 0.0
+            where = p.table[k].peers if peers else p.table[k].grad
+            hip.memcpy_htod(where + at * SIZE[grad], encode(np.zeros(1), grad))
+        p.arena.image = p.arena.dev.download(np.uint8, p.arena.size)
+        grad_norm(p)
+        check_norm(p)
+    finally:
+        p.close()
 
 
 def test_empty_lists():
@@ -457,6 +486,30 @@ def test_event_pool_exhausted():
             mc.xccl_mc_event_free(ev)
         hip.stream_destroy(stream.hip_stream)
         p.close()
+
+
+def test_plan_outlives_close():
+    """close() (the dispatcher's free_cache) releases the component's streams and events; a plan is the caller's and works on."""
+    code = (
+        "import sys\n"
+        "sys.path[:0] = [%r, %r]\n"
+        "from step_util import *\n"
+        "hip.set_device(0)\n"
+        "assert mc.xccl_mem_component_init() == Status.OK\n"
+        "p = Problem([5000, 3], F32, F32, NONE, 8)\n"
+        "grad_norm(p)\n"
+        "first = p.read_stats().tobytes()\n"
+        "mc.xccl_mem_component_free_cache()\n"
+        "grad_norm(p)\n"
+        "assert p.read_stats().tobytes() == first\n"
+        "args = p.args(max_norm=1.0, use_stats=True)\n"
+        "ok(mc.xccl_mem_component_adamw_nb(p.plan.handle, args, MemType.ROCM, None, False))\n"
+        "mc.xccl_mem_component_free_cache()\n"     # waits for the step
+        "p.check_step(args, 5, stats=p.read_stats())\n"
+        "p.close()\n"
+        "print('done')\n") % (ROOT, os.path.join(ROOT, "tests"))
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100)
+    assert out.returncode == 0 and out.stdout.strip().endswith("done"), out.stdout + out.stderr
 
 
 def test_several_threads():
