@@ -4,7 +4,8 @@ The product is three shared objects under ``xccl_amd/lib`` built from
 ``xccl_amd/csrc`` (see ``xccl_amd.build``):
 
 * ``xccl_rocm_mem_component.so`` -- the plugin libxccl dlopens; C host side on
-  the HIP runtime plus hand-written gfx950 kernels;
+  the HIP runtime plus hand-written gfx950 kernels (reductions, and the
+  optimizer step on a folded gradient);
 * ``libxccl_mc.so`` -- XCCL's mem-component dispatcher, standalone;
 * ``libxccl_rocm_benchkit.so`` -- synthetic-input kernels for bench and tests.
 
