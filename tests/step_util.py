@@ -130,10 +130,10 @@ class Problem:
     """A list of tensors on the device, its plan, and what the formulas give in 64 bits."""
 
     def __init__(self, sizes, grad=F32, param=F32, copy=NONE, bits=32, peers=0, fold=None, shift=0, seed=1, magnitude=1e-3,
-                 start=None, plant=(), peer_pad=0):
+                 start=None, plant=(), peer_pad=0, params=0.05):
         """`fold`: None, "own", "grad" or "peers": where the folded gradient is written.  `shift`: elements every piece is
         moved off alignment, differently for each.  `plant`: (tensor, element, value) put into the last gradient vector.
-        `start`: "zero" for states that are all zero."""
+        `start`: "zero" for states that are all zero.  `params`: magnitude of the parameters."""
         rng = np.random.RandomState(seed)
         self.grad, self.param, self.copy, self.bits, self.peers, self.fold = grad, param, copy, bits, peers, fold
         self.arena, self.tensors = Arena(), []
@@ -155,7 +155,7 @@ class Problem:
             t.pos, pos = pos, pos + n
             t.folded = self.arena.add(encode(np.zeros(n), grad), off(SIZE[grad], 1)) if fold == "own" else None
             if bits:
-                t.p = decode(encode(rng.randn(n) * 0.05, param), param)
+                t.p = decode(encode(rng.randn(n) * params, param), param)
                 t.param = self.arena.add(encode(t.p, param), off(SIZE[param], 2))
                 t.copy = None if copy == NONE else self.arena.add(encode(np.zeros(n), copy), off(2, 3))
                 m, v = rng.randn(n) * mag * 0.3, mag * mag * (0.2 + rng.rand(n)) * 10.0 ** rng.uniform(-6, 0, n)

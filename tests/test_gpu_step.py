@@ -144,6 +144,72 @@ def test_step_folds_the_peers(bits, grad, peers):
         p.close()
 
 
+def test_most_peers():
+    p = Problem([1, 300], BF16, F32, NONE, 32, peers=mc.STEP_MAX_PEERS, fold="own")
+    try:
+        grad_norm(p)
+        values = check_norm(p)
+        p.check_step(run_step(p, grad_scale=1.0 / 256, use_folded=True), 5, folds=values)
+    finally:
+        p.close()
+
+
+@pytest.mark.parametrize("stride", [0, (1 << 32) + 68])
+def test_peer_strides(stride):
+    """The same vector as every peer's, and vectors more than 2^32 bytes apart."""
+    n, peers = 5000, 2
+    rng = np.random.RandomState(4)
+    rows = [rng.randn(n).astype(np.float32) for _ in range(1 + peers)]
+    buf = hip.DeviceBuffer((peers - 1) * stride + n * 4 + 256)
+    p = Problem([n], F32, F32, NONE, 32, peers=peers)
+    try:
+        t = p.tensors[0]
+        t.g = [r.astype(np.float64) for r in (rows if stride else [rows[0], rows[2], rows[2]])]
+        hip.memcpy_htod(p.table[0].grad, rows[0])
+        for j in range(peers):
+            buf.upload(rows[1 + j], j * stride + 4)
+        p.table[0].peers, p.layout.peer_stride = buf.ptr + 4, stride
+        p.plan.close()
+        p.plan = mc.StepPlan(p.layout, p.table)
+        grad_norm(p)
+        a, ea = p.fold_of(t)
+        slack = (n + 2) * 2.0 ** -53 + 2 * U
+        got = p.read_stats()
+        assert np.sum(np.maximum(np.abs(a) - ea, 0) ** 2) * (1 - slack) <= got[0] <= np.sum((np.abs(a) + ea) ** 2) * (1 + slack)
+        p.check_step(run_step(p), 5)
+    finally:
+        p.close()
+        buf.close()
+
+
+def test_a_fold_that_overflows_its_type():
+    """fp16 vectors whose sum has no fp16 value: infinite as written, counted, and the step that reads it is skipped."""
+    p = Problem([700], F16, F32, NONE, 32, peers=1, fold="own", magnitude=1.0, plant=[(0, 5, 40000.0), (0, 699, -60000.0)])
+    try:
+        for at, value in ((5, 40000.0), (699, -60000.0)):
+            hip.memcpy_htod(p.table[0].grad + 2 * at, encode(np.array([value]), F16))
+        grad_norm(p)
+        assert p.read_stats()[1] == 2 and np.isinf(p.read_stats()[0])
+        run_step(p, use_stats=True, use_folded=True)
+        p.arena.download()
+        folded = decode(p.arena.get(p.tensors[0].folded), F16)
+        assert folded[5] == np.inf and folded[699] == -np.inf and np.isfinite(folded[6:699]).all()
+        assert p.arena.unchanged(p.tensors[0].param)
+    finally:
+        p.close()
+
+
+@pytest.mark.parametrize("copy", [F16, BF16], ids=NAMES.get)
+def test_large_parameters(copy):
+    """Parameters beyond the copy's type: the copy is infinite there, as rounding says, and the parameter is what it is."""
+    p = Problem([3000], F32, F32, copy, 32, params=1e5)
+    try:
+        p.check_step(run_step(p), 5)
+        assert copy == BF16 or np.isinf(decode(p.arena.get(p.tensors[0].copy), copy)).any()
+    finally:
+        p.close()
+
+
 @pytest.mark.parametrize("fold", [None, "own", "grad", "peers"])
 @pytest.mark.parametrize("grad", TYPES, ids=NAMES.get)
 @pytest.mark.parametrize("peers", [1, 3, 8])
