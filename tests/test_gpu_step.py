@@ -526,6 +526,36 @@ def test_events_and_the_threads_own_stream():
         p.close()
 
 
+@pytest.mark.parametrize("grad", [F32, BF16], ids=NAMES.get)
+def test_hand_over_to_the_components_own_queue(grad):
+    """A step that has been waited for, then a reduction of what it wrote on the component's own dispatch queue, which is
+    ordered against no stream; and the reduction's result as the next step's gradient."""
+    n = 20000
+    p = Problem([n], grad, F32, NONE, 32)
+    out = hip.DeviceBuffer(n * 4)
+    lib = mc.component_lib()
+    try:
+        args = p.args()
+        for round_ in range(60):
+            adamw(p, args)
+            before = lib.xccl_rocm_direct_launch_count()
+            ok(mc.xccl_mem_component_reduce(p.table[0].param, p.table[0].exp_avg, out.ptr, n, Dt.FLOAT32, Op.SUM, MemType.ROCM))
+            assert lib.xccl_rocm_direct_launch_count() > before
+            p.arena.download()
+            t = p.tensors[0]
+            want = p.arena.get(t.param).view(np.float32) + p.arena.get(t.avg).view(np.float32)
+            assert np.array_equal(out.download(np.float32, n), want), round_
+            if grad == F32:
+                ok(mc.xccl_mem_component_reduce(p.table[0].grad, out.ptr, p.table[0].grad, n, Dt.FLOAT32, Op.MAX, MemType.ROCM))
+                grad_norm(p)
+                g = np.where(t.g[0].astype(np.float32) > want, t.g[0].astype(np.float32), want).astype(np.float64)
+                assert abs(p.read_stats()[0] - np.sum(g * g)) <= (n + 2) * 2.0 ** -53 * np.sum(g * g), round_
+                t.g[0] = g
+    finally:
+        out.close()
+        p.close()
+
+
 def test_event_pool_exhausted():
     """No event left: with a stream the error and nothing enqueued, without one the blocking entry."""
     p = Problem([1000], F32, bits=0)
