@@ -24,9 +24,9 @@
  * A whole step is skipped, nothing written and nothing counted, when the
  * `stats` it is given say that an element was not finite (or are no sum of
  * squares: negative, infinite, NaN): the usual answer to a loss scale that was
- * too large.  Without `stats` such an element goes
- * through the formulas and poisons its own parameter and states only (its
- * block's states, with states in 8 bits).
+ * too large.  Without `stats` such an element goes through the formulas and
+ * poisons its own parameter and states only (its block's states, with states
+ * in 8 bits).
  *
  * The two doubles of `stats` can be summed over ranks with the component's
  * own FLOAT64 SUM before the step reads them.
@@ -34,13 +34,13 @@
  * States in 8 bits.  A block is XCCL_ROCM_STEP_BLOCK consecutive elements of
  * one tensor (the last may be shorter) and has one 32-bit scale per state, a
  * power of two: the smallest that keeps the block's largest magnitude at or
- * below 448 of it, and no smaller than 2^-126.  exp_avg holds m / scale and exp_avg_sq holds
- * sqrt(v) / scale, each rounded to the nearest e4m3 number (4 exponent bits,
- * 3 mantissa bits, no infinities; ties to even).  sqrt(v) > 0 is never rounded to 0: its
- * code is at least the smallest, 2^-9, because a zero there would divide a
- * non-zero m by eps alone.  The parameter is updated from m and v as they
- * were before this rounding.  States that are all zero bytes, scales
- * included, are a valid start.
+ * below 448 of it, and no smaller than 2^-126.  exp_avg holds m / scale and
+ * exp_avg_sq holds sqrt(v) / scale, each rounded to the nearest e4m3 number (4
+ * exponent bits, 3 mantissa bits, no infinities; ties to even).  sqrt(v) > 0 is
+ * never rounded to 0: its code is at least the smallest, 2^-9, because a zero
+ * there would divide a non-zero m by eps alone.  The parameter is updated from
+ * m and v as they were before this rounding.  States that are all zero bytes,
+ * scales included, are a valid start.
  */
 #ifndef XCCL_ROCM_STEP_H_
 #define XCCL_ROCM_STEP_H_
@@ -75,8 +75,9 @@ typedef struct xccl_rocm_step_layout {
  * grad_norm writes the folded gradient (rounded once to grad_dtype); given for
  * all tensors or for none, only with peers, and may be exactly `grad` or
  * exactly `peers`; a step after that reads `folded` (use_folded), since the
- * vectors it would fold are no longer what they were.  Apart from that nothing that is written may overlap
- * anything else of the plan.  A tensor of size 0 is passed over.
+ * vectors it would fold are no longer what they were.  Apart from that nothing
+ * that is written may overlap anything else of the plan.  A tensor of size 0 is
+ * passed over.
  */
 typedef struct xccl_rocm_step_tensor {
     void  *grad;
@@ -121,7 +122,8 @@ typedef struct xccl_rocm_step_plan xccl_rocm_step_plan_t;
  * above do not allow, XCCL_ERR_UNSUPPORTED for a type without a kernel; says
  * on stderr which tensor), allocates, and synchronises: not inside a capture.
  * The list itself is not kept.  plan_destroy waits for the device; graphs that
- * hold calls on the plan must not run any more.  On the device a plan takes 96
+ * hold calls on the plan must not run any more, and it comes before the
+ * component is finalized, which frees no plans.  On the device a plan takes 96
  * bytes per tensor and 8 (24 without peers) per 1024 elements.
  *
  * Steps are fastest when a tensor's arrays begin on 128-byte lines; with states

@@ -448,15 +448,15 @@ __global__ void __launch_bounds__(kNormWaves * 64) grad_norm_kernel(const NormAr
 
 // With peers' vectors: a wave folds N tiles at a time, and writes the fold if
 // there is a place for it.
-constexpr int      kFoldTiles   = 2;
+constexpr int      kFoldTiles    = 2;
 constexpr uint32_t kFoldPerChunk = STEP_CHUNK / 256 / kFoldTiles;
 
 template <typename G, bool Full, int N>
 __device__ __forceinline__ void fold_tiles(const NormArgs &a, const step_entry_t &t, const Span *span, NormSum &s,
                                            uint32_t &bad)
 {
-    const uint32_t           lane = threadIdx.x & 63;
-    Fold<G, Full, true, N>   fold;
+    const uint32_t         lane = threadIdx.x & 63;
+    Fold<G, Full, true, N> fold;
     fold.begin(t.grad, t.peers, a.n_peers, a.peer_stride, span, lane);
     fold.end();
 #pragma unroll
@@ -520,12 +520,12 @@ static_assert(kStepTile == XCCL_ROCM_STEP_BLOCK, "a tile is a block of the 8-bit
 struct AdamwKernelArgs {
     const step_entry_t   *entries;
     const step_chunk_t   *chunks;
-    const step_scalars_t *from;  // device: read instead of `s` if not NULL
-    const double         *stats; // device, or NULL
+    const step_scalars_t *from;    // device: read instead of `s` if not NULL
+    const double         *stats;   // device, or NULL
     step_scalars_t        s;
     double                zero[2]; // read instead of *stats if there is none
     double                grad_scale, max_norm;
-    uint32_t              clip; // work the factor out here: there is a norm, and no clock
+    uint32_t              clip;    // work the factor out here: there is a norm, and no clock
     size_t                peer_stride;
     uint32_t              n_peers;
     uint32_t              use_folded;
@@ -743,11 +743,11 @@ __global__ void __launch_bounds__(64) adamw_kernel(const AdamwKernelArgs a)
     // All of it lies in memory that is constant meanwhile: a choice of addresses, and no branch in front of the loads.
     typedef const __attribute__((address_space(4))) char *Constant;
     const Constant args = (Constant)__builtin_amdgcn_kernarg_segment_ptr();
-    const auto     from = (const __attribute__((address_space(4))) step_scalars_t *)(
+    const auto     from  = (const __attribute__((address_space(4))) step_scalars_t *)(
         a.from != nullptr ? (Constant)a.from : args + offsetof(AdamwKernelArgs, s));
     const auto     stats = (const __attribute__((address_space(4))) uint64_t *)(
         a.stats != nullptr ? (Constant)a.stats : args + offsetof(AdamwKernelArgs, zero));
-    const bool     skip = step_skips(stats[0], stats[1]);
+    const bool     skip  = step_skips(stats[0], stats[1]);
     step_scalars_t s;
     s.lr     = from->lr;
     s.size   = from->size;

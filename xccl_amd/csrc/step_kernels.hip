@@ -56,8 +56,9 @@ AdamwKernel adamw_by_types(xccl_dt_t param, xccl_dt_t grad, bool eight, bool pee
 // bound how many share a compute unit: as many as keep 54 KiB of loads in
 // flight, one gradient vector counted (56 KiB with 8-bit states, which take
 // longer from load to store).  More of them only disturb each other's order of
-// access to memory; a step that mostly stays in the memory-side cache does not mind.  Measured, us at 0 / 6 / 7 / 8 / 10 / 12 / 16 KiB asked for (32 /
-// 26 / 22 / 20 / 16 / 13 / 10 waves):
+// access to memory; a step that mostly stays in the memory-side cache does not
+// mind.  Measured, us at 0 / 6 / 7 / 8 / 10 / 12 / 16 KiB asked for (32 / 26 /
+// 22 / 20 / 16 / 13 / 10 waves):
 //   32-bit states, all 32 bits, 256 Mi elements   1188 1207 1177 1146 1135 1115 1161
 //   32-bit states, bf16 gradient and copy, 64 Mi   310  309  303  299  297  304  325
 //   32-bit states, 3 peers, bf16 copy, 32 Mi       238  236  231  229  227  213  225
@@ -136,11 +137,11 @@ xccl_status_t step_launch_adamw(const xccl_rocm_step_plan_t *plan, const xccl_ro
     a.eps         = (float)args->eps;
     if (args->clock != nullptr) {
         ClockArgs c;
-        c.clock = args->clock;
-        c.stats = args->stats != nullptr ? args->stats : plan->zeros;
-        c.to    = plan->scalars;
-        c.beta1 = args->beta1;
-        c.beta2 = args->beta2;
+        c.clock      = args->clock;
+        c.stats      = args->stats != nullptr ? args->stats : plan->zeros;
+        c.to         = plan->scalars;
+        c.beta1      = args->beta1;
+        c.beta2      = args->beta2;
         c.grad_scale = args->grad_scale;
         c.max_norm   = args->max_norm;
         const xccl_status_t st = launch("the step's clock", (const void *)step_clock_kernel, 1, 1, &c, 0, hip_stream);
