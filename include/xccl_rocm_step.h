@@ -13,7 +13,8 @@
  *
  *   fold    a = grad + peer{0};  a = peer{j} + a,  j = 1 .. n_peers-1
  *   stats   stats[0] = sum of a^2 over all elements of all tensors,
- *           stats[1] = how many of them are infinite or NaN      (64 bits)
+ *           stats[1] = how many of them are infinite or NaN      (64 bits);
+ *           where grad_norm writes the fold, a is what it has written
  *   clip    k = min(1, max_norm / (sqrt(stats[0]) * grad_scale + 1e-6))
  *   step    g = a * (grad_scale * k)
  *           m = beta1 m + (1 - beta1) g

@@ -462,10 +462,11 @@ __device__ __forceinline__ void fold_tiles(const NormArgs &a, const step_entry_t
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         f32x4 x = fold.sum[i];
-        // rounded to the gradient's type, written or not: the norm does not depend on whether it is
+        // The step reads what is written, so the norm is that of the rounded values; what is written nowhere stays as it
+        // is in 32 bits, which is what a step that folds the vectors itself works with.
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            x[k] = (float)(G)x[k];
+            x[k] = a.writes_fold ? (float)(G)x[k] : x[k];
             s.add(x[k], k & 1);
             bad += !__builtin_isfinite(x[k]);
         }
