@@ -614,15 +614,21 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t x)
 
 // The correctly rounded square root: the hardware's is off by one unit of the
 // last place at most, and which of the three is nearest tells the sign of what
-// the product with a neighbour leaves of x (Tuckerman's test).  Below 2^-125
-// those remainders vanish and the hardware's result stays; 0 and infinity do too.
+// the product with a neighbour leaves of x (Tuckerman's test).  The remainders
+// are multiples of the product of two units of the last place, which from x =
+// 2^-102 up is at least the smallest number there is, so that none is lost.
+// Below that, and for subnormal x, which the hardware takes for 0, the root of
+// 2^64 x is taken, exactly 2^32 times as large.  0 and infinity stay what they are.
 __device__ __forceinline__ float nearest_sqrt(float x)
 {
-    const float    s     = __builtin_amdgcn_sqrtf(x);
+    const bool     small = x < 0x1p-96f;
+    const float    y     = small ? x * 0x1p64f : x;
+    const float    s     = __builtin_amdgcn_sqrtf(y);
     const uint32_t bits  = __builtin_bit_cast(uint32_t, s);
     const float    below = __builtin_bit_cast(float, bits - 1), above = __builtin_bit_cast(float, bits + 1);
-    float          r     = __builtin_fmaf(-below, s, x) <= 0 ? below : s;
-    return __builtin_fmaf(-above, s, x) > 0 ? above : r;
+    float          r     = __builtin_fmaf(-below, s, y) <= 0 ? below : s;
+    r                    = __builtin_fmaf(-above, s, y) > 0 ? above : r;
+    return small ? r * 0x1p-32f : r;
 }
 
 // The power of two that a block's values are divided by for their e4m3 codes.
