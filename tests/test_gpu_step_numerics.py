@@ -164,7 +164,7 @@ def test_roots_of_decayed_states():
 
 # ---- steps on subnormal v ----
 
-@pytest.mark.parametrize("bits", [8])
+@pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("grad", [F32, BF16], ids=NAMES.get)
 def test_step_on_the_smallest_v(grad, bits):
     """v of every exponent from the smallest 32-bit number up, and an eps that does not hide them.  Where v is subnormal its

@@ -612,22 +612,26 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t x)
     return (uint32_t)__builtin_amdgcn_readlane((int)x, 63);
 }
 
-// The correctly rounded square root: the hardware's is off by one unit of the
-// last place at most, and which of the three is nearest tells the sign of what
-// the product with a neighbour leaves of x (Tuckerman's test).  The remainders
-// are multiples of the product of two units of the last place, which from x =
-// 2^-102 up is at least the smallest number there is, so that none is lost.
-// Below that, and for subnormal x, which the hardware takes for 0, the root of
-// 2^64 x is taken, exactly 2^32 times as large.  0 and infinity stay what they are.
-__device__ __forceinline__ float nearest_sqrt(float x)
+// The square root, within one unit of the last place, or (Nearest) correctly
+// rounded: the hardware's is off by one unit at most, and which of the three is
+// nearest tells the sign of what the product with a neighbour leaves of x
+// (Tuckerman's test).  The remainders are multiples of the product of two units
+// of the last place, which from x = 2^-102 up is at least the smallest number
+// there is, so that none is lost.  Below that, and for subnormal x, which the
+// hardware takes for 0, the root of 2^64 x is taken, exactly 2^32 times as
+// large.  0 and infinity stay what they are.
+template <bool Nearest> __device__ __forceinline__ float square_root(float x)
 {
-    const bool     small = x < 0x1p-96f;
-    const float    y     = small ? x * 0x1p64f : x;
-    const float    s     = __builtin_amdgcn_sqrtf(y);
-    const uint32_t bits  = __builtin_bit_cast(uint32_t, s);
-    const float    below = __builtin_bit_cast(float, bits - 1), above = __builtin_bit_cast(float, bits + 1);
-    float          r     = __builtin_fmaf(-below, s, y) <= 0 ? below : s;
-    r                    = __builtin_fmaf(-above, s, y) > 0 ? above : r;
+    const bool  small = x < 0x1p-96f;
+    const float y     = small ? x * 0x1p64f : x;
+    float       r     = __builtin_amdgcn_sqrtf(y);
+    if constexpr (Nearest) {
+        const float    s     = r;
+        const uint32_t bits  = __builtin_bit_cast(uint32_t, s);
+        const float    below = __builtin_bit_cast(float, bits - 1), above = __builtin_bit_cast(float, bits + 1);
+        r = __builtin_fmaf(-below, s, y) <= 0 ? below : s;
+        r = __builtin_fmaf(-above, s, y) > 0 ? above : r;
+    }
     return small ? r * 0x1p-32f : r;
 }
 
@@ -716,10 +720,9 @@ __device__ __forceinline__ void adamw_tile(const AdamwKernelArgs &a, const step_
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const float vk = v[k];
-        // The hardware's square root and reciprocal are within one unit of the last place, two roundings of the many
-        // that the parameter sees.  The square root that is stored as a code is the correctly rounded one: a block's
-        // scale hangs on it.
-        r[k] = Eight ? nearest_sqrt(vk) : __builtin_amdgcn_sqrtf(vk);
+        // One unit of the last place of the root and of the hardware's reciprocal are two roundings of the many that the
+        // parameter sees.  The root that is stored as a code is the nearest one: a block's scale hangs on it.
+        r[k] = square_root<Eight>(vk);
         const float u = m[k] * __builtin_amdgcn_rcpf(__builtin_fmaf(r[k], s.inv_c2, a.eps));
         p[k]          = __builtin_fmaf(-s.size, u, p[k] * keep);
     }
