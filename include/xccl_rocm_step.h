@@ -94,8 +94,8 @@ typedef struct xccl_rocm_step_tensor {
     double weight_decay;
 } xccl_rocm_step_tensor_t;
 
-/* Step number and learning rate in device memory: for steps that are captured
- * into a graph, and for steps that may be skipped. */
+/* Step number and learning rate in memory that the device reads: for steps that
+ * are captured into a graph, and for steps that may be skipped. */
 typedef struct xccl_rocm_step_clock {
     double   lr;
     uint64_t steps; /* steps done so far; a step that is not skipped adds 1 */
@@ -106,8 +106,8 @@ typedef struct xccl_rocm_adamw_args {
     double   grad_scale;  /* of every folded gradient, e.g. 1 / (ranks * loss scale) */
     double   max_norm;    /* > 0: clip to this norm of the scaled gradient (needs stats); 0: do not clip */
     uint64_t step;        /* number of this step, from 1 */
-    const double           *stats; /* device; what grad_norm wrote, or NULL */
-    xccl_rocm_step_clock_t *clock; /* device; replaces lr and step, or NULL */
+    const double           *stats; /* what grad_norm wrote, or NULL */
+    xccl_rocm_step_clock_t *clock; /* replaces lr and step, or NULL */
     int      use_folded;  /* 1: the gradient is what grad_norm wrote to `folded`, not grad and peers */
 } xccl_rocm_adamw_args_t;
 
@@ -137,6 +137,9 @@ typedef struct xccl_rocm_step_plan xccl_rocm_step_plan_t;
  * reduce_multi_nb.  With event == NULL they may be captured into a graph;
  * grad_norm is one kernel, adamw one, or two with a clock.  Results of equal
  * inputs are equal bit for bit on one device.
+ *
+ * `stats` (two doubles) and `clock` are memory of the plan's device, managed
+ * memory, or pinned host memory; anything else is XCCL_ERR_INVALID_PARAM.
  *
  * Calls on one plan have to be ordered by the caller: they share its scratch
  * memory, and adamw writes its tensors.  That goes for graphs that hold such

@@ -1,0 +1,79 @@
+"""What the optimizer step's entries do with a plan in hand, without a GPU: mc_step.c over a stand-in for the device
+(tests/step_harness.c), so that a call which should have been refused launches nothing."""
+import ctypes
+import os
+import subprocess
+
+import pytest
+
+from xccl_amd import mc
+from xccl_amd.types import Dt, Status
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+CSRC = os.path.join(ROOT, "xccl_amd", "csrc")
+F32, NONE = int(Dt.FLOAT32), int(Dt.UNSUPPORTED)
+INVALID = Status.ERR_INVALID_PARAM
+MB, GB = 1 << 20, 1 << 30
+DEVICE, PINNED, OTHER_DEVICE = (0x7F0000000000 + k * GB for k in range(3))
+
+
+@pytest.fixture(scope="module")
+def lib(tmp_path_factory):
+    out = str(tmp_path_factory.mktemp("step") / "libstep_harness.so")
+    subprocess.run(["gcc", "-shared", "-fPIC", "-O1", "-g", "-Wall", "-Wextra", "-Werror", "-D__HIP_PLATFORM_AMD__", "-I",
+                    "/opt/rocm/include", "-I", os.path.join(ROOT, "include"), "-I", CSRC, "-o", out,
+                    os.path.join(ROOT, "tests", "step_harness.c"), os.path.join(CSRC, "mc_step.c"), "-lm",
+                    "-Wl,-Bsymbolic"], check=True)      # its own device, whatever else the process loaded
+    lib = ctypes.CDLL(out)
+    lib.harness_launches.restype = lib.harness_allocations.restype = ctypes.c_long
+    return lib
+
+
+@pytest.fixture(scope="module")
+def step(lib):
+    return ctypes.POINTER(mc.RocmStepComponent).in_dll(lib, "xccl_rocm_mem_component_step").contents
+
+
+@pytest.fixture()
+def plan(step):
+    lay = mc.StepLayout(F32, F32, NONE, 32, 0, 0)
+    table = (mc.StepTensor * 1)(mc.StepTensor(grad=DEVICE, param=DEVICE + MB, exp_avg=DEVICE + 2 * MB,
+                                              exp_avg_sq=DEVICE + 3 * MB, size=1000))
+    out = ctypes.c_void_p()
+    assert step.plan_create(ctypes.byref(lay), table, 1, ctypes.byref(out)) == Status.OK
+    yield out.value
+    assert step.plan_destroy(out) == Status.OK
+
+
+def entries(step, plan, stats, clock):
+    """Every entry that takes these pointers: (name, call)."""
+    args = mc.AdamwArgs(lr=1e-3, beta1=0.9, beta2=0.95, eps=1e-8, grad_scale=1.0, step=1, stats=stats, clock=clock)
+    out = [("adamw", lambda: step.adamw(plan, ctypes.byref(args))),
+           ("adamw_nb", lambda: step.adamw_nb(plan, ctypes.byref(args), None, None))]
+    if clock is None:
+        out += [("grad_norm", lambda: step.grad_norm(plan, stats)),
+                ("grad_norm_nb", lambda: step.grad_norm_nb(plan, stats, None, None))]
+    return out
+
+
+HOST = ctypes.create_string_buffer(64)
+
+
+@pytest.mark.parametrize("which", ["stats", "clock"])
+@pytest.mark.parametrize("where", [(ctypes.addressof(HOST) + 15) // 16 * 16, 0x1000, 2 ** 64 - 8, OTHER_DEVICE, OTHER_DEVICE + MB,
+                                   DEVICE - 8, OTHER_DEVICE + GB - 8], ids=hex)
+def test_stats_and_clock_that_the_device_cannot_reach(lib, step, plan, which, where):
+    """Plain host memory, no memory at all, memory of another device, and 16 bytes that begin before or end behind it."""
+    before = lib.harness_launches()
+    for name, call in entries(step, plan, where if which == "stats" else DEVICE + 8 * MB, where if which == "clock" else None):
+        assert call() == INVALID, name
+    assert lib.harness_launches() == before
+
+
+@pytest.mark.parametrize("where", [DEVICE, DEVICE + GB - 16, PINNED, PINNED + GB - 16], ids=hex)
+def test_stats_and_clock_that_it_can_reach(lib, step, plan, where):
+    """Device memory to its last byte, and pinned host memory."""
+    before, calls = lib.harness_launches(), entries(step, plan, where, None) + entries(step, plan, where, where)
+    for name, call in calls:
+        assert call() == Status.OK, name
+    assert lib.harness_launches() == before + len(calls) == before + 6

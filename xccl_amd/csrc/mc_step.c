@@ -169,25 +169,43 @@ static int step_check_overlap(step_ranges_t *r)
     return 1;
 }
 
+/* Whether kernels on `device` may touch the byte at p: memory of that device, managed, or (`pinned`) of the host and at
+ * the same address for the device. */
+static int step_reaches(int device, uintptr_t p, int pinned)
+{
+    hipPointerAttribute_t a;
+
+    if (hipPointerGetAttributes(&a, (void *)p) != hipSuccess) {
+        (void)hipGetLastError();
+        return 0;
+    }
+    return a.type == hipMemoryTypeManaged || a.isManaged || (a.type == hipMemoryTypeDevice && a.device == device) ||
+           (pinned && a.type == hipMemoryTypeHost && (uintptr_t)a.devicePointer == p);
+}
+
 /* First and last byte of every range are memory that the current device may touch. */
 static int step_check_memory(const step_ranges_t *r, int device)
 {
     size_t i;
-    int    end;
 
     for (i = 0; i < r->used; i++) {
-        for (end = 0; end < 2; end++) {
-            const uintptr_t       p = end ? r->at[i].hi - 1 : r->at[i].lo;
-            hipPointerAttribute_t a;
-
-            if (hipPointerGetAttributes(&a, (void *)p) != hipSuccess ||
-                !(a.type == hipMemoryTypeManaged || a.isManaged || (a.type == hipMemoryTypeDevice && a.device == device))) {
-                (void)hipGetLastError();
-                fprintf(stderr, "xccl mc_rocm: step plan: `%s` of tensor %zu is not memory of device %d\n",
-                        r->at[i].what, r->at[i].tensor, device);
-                return 0;
-            }
+        if (!step_reaches(device, r->at[i].lo, 0) || !step_reaches(device, r->at[i].hi - 1, 0)) {
+            fprintf(stderr, "xccl mc_rocm: step plan: `%s` of tensor %zu is not memory of device %d\n", r->at[i].what,
+                    r->at[i].tensor, device);
+            return 0;
         }
+    }
+    return 1;
+}
+
+/* `stats` or `clock` of a call, 16 bytes that its kernels read or write. */
+static int step_check_words(const char *what, const void *ptr, int device)
+{
+    const uintptr_t p = (uintptr_t)ptr, last = p + 15;
+
+    if (last < p || !step_reaches(device, p, 1) || !step_reaches(device, last, 1)) {
+        fprintf(stderr, "xccl mc_rocm: step: `%s` at %p is not memory of device %d\n", what, ptr, device);
+        return 0;
     }
     return 1;
 }
@@ -445,6 +463,9 @@ static xccl_status_t step_grad_norm(xccl_rocm_step_plan_t *plan, double *stats, 
         return XCCL_ERR_INVALID_PARAM;
     }
     st = step_check_device(plan);
+    if (st == XCCL_OK && !step_check_words("stats", stats, plan->device)) {
+        st = XCCL_ERR_INVALID_PARAM;
+    }
     return st != XCCL_OK ? st : mc_rocm_enqueue(step_enqueue_norm, &call, stream, event, want_sync);
 }
 
@@ -472,6 +493,10 @@ static xccl_status_t step_adamw(xccl_rocm_step_plan_t *plan, const xccl_rocm_ada
         return XCCL_ERR_INVALID_PARAM;
     }
     st = step_check_device(plan);
+    if (st == XCCL_OK && ((a->stats != NULL && !step_check_words("stats", a->stats, plan->device)) ||
+                          (a->clock != NULL && !step_check_words("clock", a->clock, plan->device)))) {
+        st = XCCL_ERR_INVALID_PARAM;
+    }
     return st != XCCL_OK ? st : mc_rocm_enqueue(step_enqueue_adamw, &call, stream, event, want_sync);
 }
 
