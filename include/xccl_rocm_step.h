@@ -122,10 +122,12 @@ typedef struct xccl_rocm_step_plan xccl_rocm_step_plan_t;
  * plan_create checks the list (XCCL_ERR_INVALID_PARAM for what the comments
  * above do not allow, XCCL_ERR_UNSUPPORTED for a type without a kernel; says
  * on stderr which tensor), allocates, and synchronises: not inside a capture.
- * The list itself is not kept.  plan_destroy waits for the device; graphs that
- * hold calls on the plan must not run any more, and it comes before the
- * component is finalized, which frees no plans.  On the device a plan takes 96
- * bytes per tensor and 8 (24 without peers) per 1024 elements.
+ * The list itself is not kept.  plan_destroy waits for the device, may be called
+ * while some stream is being captured, and leaves the plan as it was if it
+ * returns an error; graphs that hold calls on the plan must not run any more, and
+ * it comes before the component is finalized, which frees no plans.  On the
+ * device a plan takes 96 bytes per tensor and 8 (24 without peers) per 1024
+ * elements.
  *
  * Steps are fastest when a tensor's arrays begin on 128-byte lines; with states
  * in 32 bits it is enough that they all begin at the same place of one, as

@@ -78,3 +78,32 @@ def test_stats_and_clock_in_pinned_host_memory(bits):
     finally:
         hip.host_free(at)
         p.close()
+
+
+def test_a_plan_is_destroyed_while_a_stream_is_captured():
+    """By its owner or by garbage collection, whenever that comes: the capture goes on, in every mode."""
+    p = Problem([5000], F32, bits=0)
+    stream = mc.Stream(hip.stream_create())
+    try:
+        grad_norm(p)
+        want = p.read_stats().tobytes()
+        for mode in (0, 1, 2):                               # global, thread-local, relaxed
+            first, second = mc.StepPlan(p.layout, p.table), mc.StepPlan(p.layout, p.table)
+            p.set_stats(-1.0, -1.0)
+            hip.stream_begin_capture(stream.hip_stream, mode)
+            ok(mc.xccl_mem_component_grad_norm_nb(p.plan.handle, p.stats, MemType.ROCM, stream, False))
+            first.close()
+            assert first.handle is None
+            del second
+            graph = hip.stream_end_capture(stream.hip_stream)
+            run = hip.graph_instantiate(graph)
+            for _ in range(3):
+                hip.graph_launch(run, stream.hip_stream)
+                hip.stream_synchronize(stream.hip_stream)
+                assert p.read_stats().tobytes() == want, mode
+                p.set_stats(-1.0, -1.0)
+            hip.graph_destroy(graph, run)
+    finally:
+        hip.stream_synchronize(stream.hip_stream)
+        hip.stream_destroy(stream.hip_stream)
+        p.close()

@@ -77,3 +77,53 @@ def test_stats_and_clock_that_it_can_reach(lib, step, plan, where):
     for name, call in calls:
         assert call() == Status.OK, name
     assert lib.harness_launches() == before + len(calls) == before + 6
+
+
+def test_a_plan_that_cannot_be_freed_stays(lib, step):
+    """An error of the runtime leaves the plan as it was: usable, and destroyed by the next try."""
+    lay = mc.StepLayout(F32, NONE, NONE, 0, 0, 0)
+    table = (mc.StepTensor * 1)(mc.StepTensor(grad=DEVICE, size=1000))
+    out = ctypes.c_void_p()
+    before = lib.harness_allocations()
+    assert step.plan_create(ctypes.byref(lay), table, 1, ctypes.byref(out)) == Status.OK
+    try:
+        lib.harness_fail_free(900)                       # hipErrorStreamCaptureUnsupported
+        assert step.plan_destroy(out) == Status.ERR_NO_MESSAGE
+        assert lib.harness_allocations() == before + 1
+        # looked at without being called, which a plan that is gone would not survive
+        assert mc.StepLayout.from_address(out.value).grad_dtype == F32
+    finally:
+        lib.harness_fail_free(0)
+    assert step.grad_norm(out, DEVICE + MB) == Status.OK
+    assert step.plan_destroy(out) == Status.OK
+    assert lib.harness_allocations() == before
+
+
+def test_freeing_leaves_captures_alone(lib, step):
+    """The runtime's free would invalidate any capture that is going on: it runs in the relaxed mode, which is put back."""
+    lay = mc.StepLayout(F32, NONE, NONE, 0, 0, 0)
+    table = (mc.StepTensor * 1)(mc.StepTensor(grad=DEVICE, size=1000))
+    out = ctypes.c_void_p()
+    assert step.plan_create(ctypes.byref(lay), table, 1, ctypes.byref(out)) == Status.OK
+    before = lib.harness_mode()
+    assert step.plan_destroy(out) == Status.OK
+    assert lib.harness_mode_at_free() == 2 and lib.harness_mode() == before == 0
+
+
+def test_close_says_so(monkeypatch):
+    """StepPlan.close() on a plan that could not be destroyed: an exception, and the handle is kept for another try."""
+    results = [Status.ERR_NO_MESSAGE, Status.OK]
+    seen = []
+
+    def destroy(handle, mem_type):
+        seen.append(handle)
+        return results[len(seen) - 1]
+    monkeypatch.setattr(mc, "xccl_mem_component_step_plan_create", lambda *a: (Status.OK, 0x1230))
+    monkeypatch.setattr(mc, "xccl_mem_component_step_plan_destroy", destroy)
+    plan = mc.StepPlan(mc.StepLayout(), [])
+    with pytest.raises(RuntimeError, match="step_plan_destroy"):
+        plan.close()
+    assert plan.handle == 0x1230
+    plan.close()
+    plan.close()                                         # nothing left to do
+    assert plan.handle is None and seen == [0x1230, 0x1230]

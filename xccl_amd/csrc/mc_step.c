@@ -404,17 +404,24 @@ static xccl_status_t mc_step_plan_create(const xccl_rocm_step_layout_t *layout, 
 
 static xccl_status_t mc_step_plan_destroy(xccl_rocm_step_plan_t *plan)
 {
-    hipError_t e;
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    hipError_t           e, swapped;
 
     if (plan == NULL) {
         return XCCL_ERR_INVALID_PARAM;
     }
-    e = hipFree(plan->memory); /* waits for the device */
-    free(plan);
+    /* In the thread's usual mode hipFree is an error while any stream of the process is being captured, and invalidates
+     * that capture, which need not have anything to do with the plan. */
+    swapped = hipThreadExchangeStreamCaptureMode(&mode);
+    e       = hipFree(plan->memory); /* waits for the device */
+    if (swapped == hipSuccess) {
+        (void)hipThreadExchangeStreamCaptureMode(&mode);
+    }
     if (e != hipSuccess && e != hipErrorDeinitialized) {
         (void)hipGetLastError();
-        return XCCL_ERR_NO_MESSAGE;
+        return XCCL_ERR_NO_MESSAGE; /* the plan is as it was */
     }
+    free(plan);
     return XCCL_OK;
 }
 

@@ -418,7 +418,9 @@ class StepPlan:
 
     def close(self):
         if self.handle:
-            xccl_mem_component_step_plan_destroy(self.handle, self.mem_type)
+            st = xccl_mem_component_step_plan_destroy(self.handle, self.mem_type)
+            if st != Status.OK:
+                raise RuntimeError("xccl_mem_component_step_plan_destroy: %s" % st)
             self.handle = None
 
     def __del__(self):
