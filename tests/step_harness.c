@@ -26,6 +26,8 @@ long harness_allocations(void) { return allocations; }
 void harness_fail_free(int error) { free_result = (hipError_t)error; }
 int  harness_mode_at_free(void) { return mode_at_free; }
 int  harness_mode(void) { return capture_mode; }
+unsigned harness_norm_grid(size_t chunks, int fold, size_t elem) { return step_norm_grid(chunks, fold, elem); }
+unsigned harness_norm_most(int fold) { return fold ? STEP_FOLD_GRID : STEP_NORM_GRID; }
 
 hipError_t hipGetDevice(int *device)
 {

@@ -127,3 +127,17 @@ def test_close_says_so(monkeypatch):
     plan.close()
     plan.close()                                         # nothing left to do
     assert plan.handle is None and seen == [0x1230, 0x1230]
+
+
+@pytest.mark.parametrize("elem", [4, 2])
+@pytest.mark.parametrize("fold", [0, 1])
+def test_no_workgroup_of_the_norm_without_work(lib, fold, elem):
+    """As many workgroups of four waves as the chunks of 1024 elements keep busy, up to the most there are.  A wave takes 4 KiB at
+    once without peers, half a chunk with them."""
+    most = lib.harness_norm_most(fold)
+    per_wave = 512 if fold else 4096 // elem                 # elements
+    for chunks in [0, 1, 2, 3, 4, 5, 7, 8, 9, 15, 16, 17, 2047, 2048, 2049, 4095, 4096, 4097, 8193, 0x1fffffff]:
+        grid = lib.harness_norm_grid(ctypes.c_size_t(chunks), fold, ctypes.c_size_t(elem))
+        waves = -(-chunks * 1024 // per_wave)
+        assert grid == max(1, min(most, -(-waves // 4))), (chunks, grid)
+        assert grid == 1 or (grid - 1) * 4 < waves            # the last workgroup has a wave with work

@@ -216,7 +216,7 @@ template <typename G, bool Full, bool Peers, int N> struct Fold {
 
 // ---- the norm ---------------------------------------------------------------
 
-constexpr uint32_t kNormWaves = 4; // of a workgroup
+constexpr uint32_t kNormWaves = STEP_NORM_WAVES;
 
 struct NormArgs {
     const step_entry_t *entries;
@@ -391,7 +391,7 @@ __device__ __forceinline__ uint32_t norm_left(const NormArgs &a, const step_piec
 template <typename G>
 __global__ void __launch_bounds__(kNormWaves * 64) grad_norm_kernel(const NormArgs a)
 {
-    constexpr uint32_t K    = 4096 / (STEP_CHUNK * sizeof(G)); // chunks at once
+    constexpr uint32_t K    = STEP_NORM_BYTES / (STEP_CHUNK * sizeof(G)); // chunks at once
     const uint32_t     wave = blockIdx.x * kNormWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t     step = a.grid * kNormWaves * K;
     NormSum            s;
@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(kNormWaves * 64) grad_norm_kernel(const NormAr
 
 // With peers' vectors: a wave folds N tiles at a time, and writes the fold if
 // there is a place for it.
-constexpr int      kFoldTiles    = 2;
+constexpr int      kFoldTiles    = STEP_FOLD_TILES;
 constexpr uint32_t kFoldPerChunk = STEP_CHUNK / 256 / kFoldTiles;
 
 template <typename G, bool Full, int N>

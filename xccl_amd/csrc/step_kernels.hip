@@ -99,11 +99,7 @@ xccl_status_t step_launch_grad_norm(const xccl_rocm_step_plan_t *plan, double *s
     a.n_chunks    = (uint32_t)plan->chunks;
     a.n_peers     = plan->layout.n_peers;
     a.writes_fold = plan->writes_fold;
-    // one wave for each unit of work, up to a grid that is resident at once and then goes round
-    const uint32_t units = fold ? a.n_chunks * kFoldPerChunk : a.n_chunks;
-    const uint32_t want  = (units + kNormWaves - 1) / kNormWaves;
-    const uint32_t most  = fold ? STEP_FOLD_GRID : STEP_NORM_GRID;
-    a.grid               = want < 1 ? 1 : want < most ? want : most;
+    a.grid        = step_norm_grid(plan->chunks, fold, plan->layout.grad_dtype == XCCL_DT_FLOAT32 ? 4 : 2);
     const void *fn;
     switch ((int)plan->layout.grad_dtype) {
     case XCCL_DT_FLOAT32: fn = fold ? (const void *)fold_norm_kernel<float> : (const void *)grad_norm_kernel<float>; break;

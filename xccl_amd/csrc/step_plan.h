@@ -47,6 +47,22 @@ typedef struct step_piece {
 /* grad_norm runs at most this many workgroups, without and with peers; each leaves one partial result. */
 #define STEP_NORM_GRID 512u
 #define STEP_FOLD_GRID 1024u
+#define STEP_NORM_WAVES 4u    /* of a workgroup */
+#define STEP_NORM_BYTES 4096u /* that a wave requests at once without peers: one chunk of 32-bit elements, two of 16-bit ones */
+#define STEP_FOLD_TILES 2u    /* of 256 elements, that a wave folds at once */
+
+/* Workgroups of grad_norm: a wave for each piece of work that it takes at once, up to a grid that is resident at once and
+ * then goes round.  A workgroup that found no work would still leave a partial result and count itself in. */
+static inline uint32_t step_norm_grid(size_t chunks, int fold, size_t elem)
+{
+    const size_t at_once = STEP_NORM_BYTES / (STEP_CHUNK * elem); /* chunks of a wave */
+    const size_t waves   = fold ? chunks * (STEP_CHUNK / 256 / STEP_FOLD_TILES) : (chunks + at_once - 1) / at_once;
+    const size_t want    = (waves + STEP_NORM_WAVES - 1) / STEP_NORM_WAVES;
+    const size_t most    = fold ? STEP_FOLD_GRID : STEP_NORM_GRID;
+
+    return (uint32_t)(want < 1 ? 1 : want < most ? want : most);
+}
+
 typedef struct step_partial {
     double   sum;
     uint64_t bad;
