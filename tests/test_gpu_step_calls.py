@@ -107,3 +107,18 @@ def test_a_plan_is_destroyed_while_a_stream_is_captured():
         hip.stream_synchronize(stream.hip_stream)
         hip.stream_destroy(stream.hip_stream)
         p.close()
+
+
+def test_the_runtimes_own_streams():
+    """The legacy default stream and the per-thread one belong to the current device."""
+    p = Problem([5000], F32, F32, NONE, 32)
+    try:
+        grad_norm(p)
+        want = p.read_stats().tobytes()
+        for handle in (0, 1, 2):                              # default, legacy, per thread
+            p.set_stats(-1.0, -1.0)
+            ok(mc.xccl_mem_component_grad_norm_nb(p.plan.handle, p.stats, MemType.ROCM, mc.Stream(handle), False))
+            hip.device_synchronize()
+            assert p.read_stats().tobytes() == want, handle
+    finally:
+        p.close()
