@@ -122,3 +122,30 @@ def test_the_runtimes_own_streams():
             assert p.read_stats().tobytes() == want, handle
     finally:
         p.close()
+
+
+def test_destroying_a_plan_waits_for_its_calls():
+    """A plan that is closed behind a call which still runs: the call is complete when close() returns."""
+    n = 1 << 26
+    buf = hip.DeviceBuffer(16 * n)
+    hip.memset(buf.ptr, 0, 16 * n)
+    e = mc.StepTensor(grad=buf.ptr, param=buf.ptr + 4 * n, exp_avg=buf.ptr + 8 * n, exp_avg_sq=buf.ptr + 12 * n, size=n)
+    args = mc.AdamwArgs(lr=1.0, beta1=0.5, beta2=0.5, eps=1.0, grad_scale=1.0, step=1)
+    stream = mc.Stream(hip.stream_create())
+    try:
+        for k, one in enumerate((None, stream)):
+            ones = np.full(16, float(k + 1), np.float32)
+            buf.upload(ones, 4 * (n - 16))
+            plan = mc.StepPlan(mc.StepLayout(F32, F32, NONE, 32, 0, 0), [e])
+            for _ in range(8):
+                ok(mc.xccl_mem_component_adamw_nb(plan.handle, args, MemType.ROCM, one, False))
+            plan.close()
+            m = buf.download(np.float32, 16, 12 * n - 64)
+            if k == 0:
+                assert (m == 1 - 2.0 ** -8).all()            # m = 0.5 m + 0.5, eight times
+            else:
+                assert (m == 2 - 2.0 ** -8 * (2 - (1 - 2.0 ** -8))).all()
+    finally:
+        hip.stream_synchronize(stream.hip_stream)
+        hip.stream_destroy(stream.hip_stream)
+        buf.close()
