@@ -101,6 +101,10 @@ typedef struct xccl_rocm_step_clock {
     uint64_t steps; /* steps done so far; a step that is not skipped adds 1 */
 } xccl_rocm_step_clock_t;
 
+/* 0 <= beta1, beta2 < 1.  eps and grad_scale are positive normal 32-bit numbers
+ * (from 1.2e-38): eps = 0, which would divide 0 by 0 where m and v are, and a
+ * gradient that is switched off or negated by its scale are refused.  lr and
+ * max_norm are finite and not negative.  What a clock holds is not looked at. */
 typedef struct xccl_rocm_adamw_args {
     double   lr, beta1, beta2, eps;
     double   grad_scale;  /* of every folded gradient, e.g. 1 / (ranks * loss scale) */

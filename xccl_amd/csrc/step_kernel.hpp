@@ -28,9 +28,9 @@ typedef uint32_t u32x4s __attribute__((ext_vector_type(4)));
 
 // Cache policy: loads nt; stores written through (sc0 sc1) or nt.  With 32-bit
 // gradients writing through is faster, with 16-bit ones nt is.  Measured, step,
-// written through / nt, us: 32-bit gradients, 32-bit states 256 Mi 1112 / 1135, 3
-// peers 32 Mi 215 / 221, 8-bit states 256 Mi 640 / 658; 16-bit gradients, 32-bit
-// states 64 Mi 299 / 290, 8-bit states 64 Mi 177 / 173, 1 peer 24 Mi 52 / 51.
+// written through / nt, us: 32-bit gradients, 32-bit states 256 Mi 1111 / 1147, 3
+// peers 32 Mi 216 / 223, 8-bit states 256 Mi 650 / 663; 16-bit gradients, 32-bit
+// states 64 Mi 300 / 292, 8-bit states 64 Mi 177 / 175, 1 peer 24 Mi 53 / 52.
 constexpr int kStepAuxLoad = 0x02;
 template <typename G> constexpr int kStepAuxStore = sizeof(G) == 4 ? 0x11 : 0x02;
 
@@ -163,9 +163,13 @@ __device__ __forceinline__ void store_codes(char *p, const Span &s, uint32_t lan
 }
 
 // a = grad + peer{0}; a = peer{j} + a: reduce_multi's order, in 32 bits whatever
-// the gradient's type, N tiles at once.  As there the vectors are walked one by
-// one with two in flight; the last of them is requested by begin and added by
-// end, so that the caller can request what else it needs in between.
+// the gradient's type, N tiles at once.  The vectors are walked one by one, and a
+// wave has one of the peers' in flight at a time: with 32-bit elements a round of
+// the loop begins or ends with a wait for all loads, with 16-bit ones, which are
+// converted where they are requested, every request is waited for at once.  Other
+// waves have to cover that.  The last 32-bit vector is requested by begin and
+// added by end, so that what the caller requests in between goes out with it; with
+// 16-bit elements the caller's requests come behind the whole fold.
 template <typename G, bool Full, bool Peers, int N> struct Fold {
     f32x4 sum[N], more[Peers ? N : 1];
 

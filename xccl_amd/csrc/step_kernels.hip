@@ -59,13 +59,13 @@ AdamwKernel adamw_by_types(xccl_dt_t param, xccl_dt_t grad, bool eight, bool pee
 // access to memory; a step that mostly stays in the memory-side cache does not
 // mind.  Measured, us at 0 / 6 / 7 / 8 / 10 / 12 / 16 KiB asked for (32 / 26 /
 // 22 / 20 / 16 / 13 / 10 waves):
-//   32-bit states, all 32 bits, 256 Mi elements   1188 1207 1177 1146 1135 1115 1161
-//   32-bit states, bf16 gradient and copy, 64 Mi   310  309  303  299  297  304  325
-//   32-bit states, 3 peers, bf16 copy, 32 Mi       238  236  231  229  227  213  225
-//   8-bit states, 32-bit gradient, 256 Mi          712  675  643  665  695  816  996
-//   8-bit states, bf16 gradient and copy, 64 Mi    175  174  182  194  202  237  284
-//   8-bit states, bf16, 1 peer, 24 Mi (200 MB)      52   56   62   68   74   90  113
-//   32-bit states, fp16, 8 Mi (100 MB)              34   34   34   35   35   37   40
+//   32-bit states, all 32 bits, 256 Mi elements   1217 1229 1190 1163 1149 1111 1152
+//   32-bit states, bf16 gradient and copy, 64 Mi   307  304  299  295  293  293  300
+//   32-bit states, 3 peers, bf16 copy, 32 Mi       241  238  233  231  229  216  229
+//   8-bit states, 32-bit gradient, 256 Mi          718  671  646  674  707  834 1019
+//   8-bit states, bf16 gradient and copy, 64 Mi    174  175  175  181  188  217  266
+//   8-bit states, bf16, 1 peer, 24 Mi (200 MB)      52   56   61   67   73   89  111
+//   32-bit states, fp16, 8 Mi (100 MB)              32   31   31   32   32   33   35
 unsigned adamw_lds(const xccl_rocm_step_plan_t *plan, uint32_t n_peers)
 {
     const xccl_rocm_step_layout_t &l       = plan->layout;
